@@ -257,6 +257,68 @@ int mlstm_chunk_sp_apply(const void* q, const void* k, const void* v, const void
                          int rank, void* h, int h_dtype, double* carry_out, void* workspace, size_t workspace_bytes,
                          int B, int NH, int S, int D, int dtype, int chunk, void* stream);
 
+/* Operators around the mixer: the short convolution in front of it, a selective state space scan as a mixer of its own, and
+ * the norm with the residual's addition.  The reference has none of them.  Their kernels have no internal waits: their
+ * workspaces carry no status word, and a workspace of 0 bytes may be NULL.  Pointers need the alignment of their elements only
+ * (16 bytes for workspaces, 8 for checkpoints); where everything is aligned to 16 bytes, wider accesses are used.  Sums are
+ * fp32 and taken in a fixed order (no atomics): the same call gives the same bits.
+ *
+ * Short causal convolution, channel by channel: y_t = act(bias + sum_k weight[c][k] x_{t-(W-1)+k}), W = 2, 3 or 4, act = silu or
+ * none.  x [B,S,C] with element strides {batch, position} in `strides` (a host array; NULL: contiguous), y [B,S,C] contiguous;
+ * weight [C,W] and bias [C] (or NULL) of `w_dtype`: the inputs' type or float32.
+ *   initial [B,W-1,C]    the inputs in front of position 0, or NULL (zeros)
+ *   state_out [B,W-1,C]  the last W-1 inputs of the call (and of `initial` where S < W-1), or NULL; may be `initial` itself
+ * Backward (of a call with no `initial`): dy, dx [B,S,C] contiguous, dweight, dbias of `w_dtype` (dbias NULL as bias is). */
+int mlstm_conv_fwd(const void* x, const void* weight, const void* bias, const void* initial, const long long* strides, void* y,
+                   void* state_out, int B, int S, int C, int W, int dtype, int w_dtype, int silu, void* stream);
+size_t mlstm_conv_bwd_workspace(int B, int S, int C, int W, int dtype);
+int mlstm_conv_bwd(const void* dy, const void* x, const void* weight, const void* bias, const long long* strides, void* dx,
+                   void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int B, int S, int C, int W, int dtype,
+                   int w_dtype, int silu, void* stream);
+
+/* Selective state space scan.  Per channel c of group g = c / (C / G), with N <= 64 states:
+ *   delta_t = softplus(dt_t + dt_bias)  (softplus = 0: dt_t + dt_bias)
+ *   h_t[n]  = exp(delta_t A[c][n]) h_{t-1}[n] + delta_t x_t Bv_t[g][n]
+ *   y_t     = (sum_n Cv_t[g][n] h_t[n] + D[c] x_t) * silu(z_t)
+ * x, dt, z [B,S,C], Bv, Cv [B,S,G,N] of `dtype`, the last (two) dimension(s) contiguous; `strides` (host, NULL: contiguous):
+ * element strides {batch, position} of x, dt, Bv, Cv, z.  A [C,N], D [C], dt_bias [C] float32; D, z, dt_bias may be NULL.
+ * y [B,S,C] contiguous.  States [B,C,N] float32: `initial` (NULL: zeros), `state_out` (NULL: not wanted; may be `initial`).
+ *   checkpoints   NULL, or mlstm_ssm_checkpoint_floats() floats that the backward of the same call takes
+ * Up to mlstm_ssm_step_max_tokens() positions without checkpoints take a kernel of their own (decoding).
+ * Backward (of a call with no `initial`): dy and dx, ddt, dz [B,S,C], dB, dC [B,S,G,N] contiguous of `dtype`; dA, dD, d_dt_bias
+ * float32.  dD, dz, d_dt_bias are NULL exactly where D, z, dt_bias are.  Its workspace holds one {dB, dC} pair of floats for each
+ * 64 channels, position and state, for as many batch entries at a time as fit 512 MB. */
+int mlstm_ssm_step_max_tokens(void);
+size_t mlstm_ssm_checkpoint_floats(int B, int S, int C, int G, int N);
+size_t mlstm_ssm_fwd_workspace(int B, int S, int C, int G, int N);
+int mlstm_ssm_fwd(const void* x, const void* dt, const float* A, const void* Bv, const void* Cv, const float* D, const void* z,
+                  const float* dt_bias, const float* initial, const long long* strides, void* y, float* state_out,
+                  float* checkpoints, void* workspace, size_t workspace_bytes, int B, int S, int C, int G, int N, int dtype,
+                  int softplus, void* stream);
+size_t mlstm_ssm_bwd_workspace(int B, int S, int C, int G, int N);
+int mlstm_ssm_bwd(const void* dy, const void* x, const void* dt, const float* A, const void* Bv, const void* Cv, const float* D,
+                  const void* z, const float* dt_bias, const long long* strides, const float* checkpoints, void* dx, void* ddt,
+                  float* dA, void* dB, void* dC, float* dD, void* dz, float* d_dt_bias, void* workspace, size_t workspace_bytes,
+                  int B, int S, int C, int G, int N, int dtype, int softplus, void* stream);
+
+/* Root-mean-square norm with the residual's addition: sum = x + residual, rounded to `s_dtype`; y = sum / sqrt(mean(sum^2) + eps)
+ * * weight over the last dimension D <= 16384 of `rows` contiguous rows.
+ *   residual, sum   of `s_dtype` (the type of x, or float32), both or neither (then s_dtype = dtype)
+ *   weight          of `w_dtype`, NULL (ones), or [groups, D]: row r takes weight row (r / inner) % groups, for [B, NH, S, D]
+ *                   tensors groups = NH and inner = S; else groups = 1
+ *   scale           NULL: y of `y_dtype` (any).  Else y is 8 bits (e4m3), scale [rows, D / block] float32 with block = 32, 64, 128 or
+ *                   D (which divides D), each the largest magnitude of its block / 448 (1 for a block of zeros): y * scale is the
+ *                   result.  block = 0 without scale.
+ * Backward: s is the sum (x where there was no residual) of `s_dtype`, dy of `dy_dtype` (s_dtype, or any where s_dtype is float32), ds
+ * of `s_dtype` the gradient of the sum from its later uses or NULL; dx of `x_dtype`; dres of `s_dtype` or NULL (the same values as
+ * dx); dweight of `w_dtype` (NULL as weight is; the workspace is needed for it only). */
+int mlstm_rms_fwd(const void* x, const void* residual, const void* weight, void* y, void* sum, float* scale, long long rows, int D,
+                  int groups, int inner, int block, float eps, int dtype, int s_dtype, int w_dtype, int y_dtype, void* stream);
+size_t mlstm_rms_bwd_workspace(long long rows, int D, int groups, int inner);
+int mlstm_rms_bwd(const void* dy, const void* ds, const void* s, const void* weight, void* dx, void* dres, void* dweight,
+                  void* workspace, size_t workspace_bytes, long long rows, int D, int groups, int inner, float eps, int x_dtype,
+                  int s_dtype, int w_dtype, int dy_dtype, void* stream);
+
 /* Copies the workspace's device status word to *host_status after synchronising `stream`.
  * Returns MLSTM_OK, or MLSTM_E_TIMEOUT when the word is non-zero, or MLSTM_E_CUDA. */
 int mlstm_read_status(const void* workspace, int* host_status, void* stream);

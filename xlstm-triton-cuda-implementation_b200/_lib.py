@@ -3,6 +3,7 @@
 torch is used for device memory and streams only: every call hands raw device pointers and the
 current CUDA stream to the library.  There is no fallback: a missing library or a failed call raises.
 """
+import contextlib
 import ctypes
 import os
 
@@ -108,6 +109,31 @@ def lib():
     L.mlstm_ogate_fwd.argtypes = [vp, vp, vp, ctypes.c_longlong, i32, i32, vp]
     L.mlstm_ogate_bwd.restype = i32
     L.mlstm_ogate_bwd.argtypes = [vp] * 5 + [ctypes.c_longlong, i32, i32, vp]
+    i64 = ctypes.c_longlong
+    L.mlstm_conv_fwd.restype = i32
+    L.mlstm_conv_fwd.argtypes = [vp] * 7 + [i32] * 7 + [vp]
+    L.mlstm_conv_bwd_workspace.restype = sz
+    L.mlstm_conv_bwd_workspace.argtypes = [i32] * 5
+    L.mlstm_conv_bwd.restype = i32
+    L.mlstm_conv_bwd.argtypes = [vp] * 8 + [vp, sz] + [i32] * 7 + [vp]
+    L.mlstm_ssm_step_max_tokens.restype = i32
+    L.mlstm_ssm_step_max_tokens.argtypes = []
+    L.mlstm_ssm_checkpoint_floats.restype = sz
+    L.mlstm_ssm_checkpoint_floats.argtypes = [i32] * 5
+    L.mlstm_ssm_fwd_workspace.restype = sz
+    L.mlstm_ssm_fwd_workspace.argtypes = [i32] * 5
+    L.mlstm_ssm_fwd.restype = i32
+    L.mlstm_ssm_fwd.argtypes = [vp] * 13 + [vp, sz] + [i32] * 7 + [vp]
+    L.mlstm_ssm_bwd_workspace.restype = sz
+    L.mlstm_ssm_bwd_workspace.argtypes = [i32] * 5
+    L.mlstm_ssm_bwd.restype = i32
+    L.mlstm_ssm_bwd.argtypes = [vp] * 19 + [vp, sz] + [i32] * 7 + [vp]
+    L.mlstm_rms_fwd.restype = i32
+    L.mlstm_rms_fwd.argtypes = [vp] * 6 + [i64] + [i32] * 4 + [ctypes.c_float] + [i32] * 4 + [vp]
+    L.mlstm_rms_bwd_workspace.restype = sz
+    L.mlstm_rms_bwd_workspace.argtypes = [i64] + [i32] * 3
+    L.mlstm_rms_bwd.restype = i32
+    L.mlstm_rms_bwd.argtypes = [vp] * 7 + [vp, sz, i64] + [i32] * 3 + [ctypes.c_float] + [i32] * 4 + [vp]
     L.mlstm_selftest_register_split.restype = i32
     L.mlstm_selftest_register_split.argtypes = [i32]
     L.mlstm_selftest_wait_timeout.restype = i32
@@ -129,6 +155,9 @@ EXPORTS = [
     "mlstm_chunk_read_mb", "mlstm_chunk_bwd_workspace", "mlstm_chunk_bwd",
     "mlstm_step_max_tokens", "mlstm_step", "mlstm_forward_f16_static_status", "mlstm_selftest_wait_timeout", "mlstm_selftest_register_split",
     "mlstm_ogate_fwd", "mlstm_ogate_bwd",
+    "mlstm_conv_fwd", "mlstm_conv_bwd_workspace", "mlstm_conv_bwd", "mlstm_ssm_step_max_tokens", "mlstm_ssm_checkpoint_floats",
+    "mlstm_ssm_fwd_workspace", "mlstm_ssm_fwd", "mlstm_ssm_bwd_workspace", "mlstm_ssm_bwd", "mlstm_rms_fwd",
+    "mlstm_rms_bwd_workspace", "mlstm_rms_bwd",
 ]
 
 
@@ -149,6 +178,34 @@ def require_cuda(*tensors):
         if not t.is_contiguous():
             raise RuntimeError("tensors must be contiguous (the reference indexes them with fixed strides)")
     return dev
+
+
+def require_one_cuda_device(first, *others):
+    """The CUDA device that all of the tensors (None: left out) live on."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise RuntimeError("these kernels need CUDA tensors; there is no CPU path")
+    for t in others:
+        if t is not None and t.device != dev:
+            raise RuntimeError("all tensors must live on the same CUDA device")
+    return dev
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(dev):
+    """``torch.cuda.device(dev)`` where another device is current, else nothing (the switch costs a few us a call)."""
+    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def scratch(nbytes: int, dev):
+    """(tensor, address, bytes) of scratch memory of one call's own.  Unlike ``workspace`` nothing is kept between calls, so a
+    captured graph owns its scratch and no later call can free or reuse it."""
+    if nbytes == 0:
+        return None, None, 0
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return buf, buf.data_ptr(), nbytes
 
 
 def stream_ptr(dev) -> int:
