@@ -5,9 +5,9 @@
 
 namespace mlstm {
 
-constexpr int RR_COLS = 32, RR_GROUPS = 8;
+constexpr int RR_COLS = 32, RR_GROUPS = 32;
 
-// out(column, sum): stores one sum.  A block takes 32 columns; eight groups of threads take every eighth row.
+// out(column, sum): stores one sum.  A block takes 32 columns; 32 groups of threads take every 32nd row.
 template <typename Out>
 __global__ void __launch_bounds__(RR_COLS * RR_GROUPS) reduce_rows_kernel(const float* __restrict__ part, int rows, long long cols, Out out) {
     __shared__ float sm[RR_GROUPS][RR_COLS];

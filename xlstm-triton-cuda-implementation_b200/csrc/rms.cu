@@ -11,6 +11,7 @@
 #include <cuda_fp8.h>
 
 #include "reduce_rows.cuh"
+#include "vec_cvt.cuh"
 
 namespace mlstm {
 namespace {
@@ -22,80 +23,30 @@ struct RmsArgs {
     long long rows;
     int D, groups, inner;           // weight row of a row: (row / inner) % groups
     int wdt, ydt, xdt, block;       // element types; block: values per scale
+    int lanes;                      // lanes of a warp per row
     float eps, inv_d;
 };
 
-// V values: 16 bytes of 16-bit values, 2 x 16 of fp32, or a single one
-template <typename T, int V>
-struct RVec {
-    T v[V];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V == 1) v[0] = *p;
-        else {
-#pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(v) / 16); i++)
-                reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
-        }
-    }
-    __device__ __forceinline__ void store(T* p) const {
-        if constexpr (V == 1) *p = v[0];
-        else {
-#pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(v) / 16); i++)
-                reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
-        }
-    }
-};
-template <typename T, int V>
-struct alignas(V == 1 ? sizeof(T) : 16) RVecA : RVec<T, V> {};
-
 template <int V>
 __device__ __forceinline__ void store_any(void* p, int dtype, long long at, const float (&f)[V]) {
-    if (dtype == MLSTM_DT_F32) {
-        RVecA<float, V> o;
-#pragma unroll
-        for (int j = 0; j < V; j++) o.v[j] = f[j];
-        o.store(static_cast<float*>(p) + at);
-    } else if (dtype == MLSTM_DT_F16) {
-        RVecA<__half, V> o;
-#pragma unroll
-        for (int j = 0; j < V; j++) o.v[j] = from_f32<__half>(f[j]);
-        o.store(static_cast<__half*>(p) + at);
-    } else {
-        RVecA<__nv_bfloat16, V> o;
-#pragma unroll
-        for (int j = 0; j < V; j++) o.v[j] = from_f32<__nv_bfloat16>(f[j]);
-        o.store(static_cast<__nv_bfloat16*>(p) + at);
-    }
+    if (dtype == MLSTM_DT_F32) store_vec<float, V>(static_cast<float*>(p) + at, from_floats<float, V>(f));
+    else if (dtype == MLSTM_DT_F16) store_vec<__half, V>(static_cast<__half*>(p) + at, from_floats<__half, V>(f));
+    else store_vec<__nv_bfloat16, V>(static_cast<__nv_bfloat16*>(p) + at, from_floats<__nv_bfloat16, V>(f));
 }
 template <int V>
 __device__ __forceinline__ void load_weight(const RmsArgs& p, long long at, float (&w)[V]) {
     if (!p.weight) {
 #pragma unroll
         for (int j = 0; j < V; j++) w[j] = 1.0f;
-    } else if (p.wdt == MLSTM_DT_F32) {
-        RVecA<float, V> r;
-        r.load(static_cast<const float*>(p.weight) + at);
-#pragma unroll
-        for (int j = 0; j < V; j++) w[j] = r.v[j];
-    } else if (p.wdt == MLSTM_DT_F16) {
-        RVecA<__half, V> r;
-        r.load(static_cast<const __half*>(p.weight) + at);
-#pragma unroll
-        for (int j = 0; j < V; j++) w[j] = to_f32<__half>(r.v[j]);
-    } else {
-        RVecA<__nv_bfloat16, V> r;
-        r.load(static_cast<const __nv_bfloat16*>(p.weight) + at);
-#pragma unroll
-        for (int j = 0; j < V; j++) w[j] = to_f32<__nv_bfloat16>(r.v[j]);
-    }
+    } else if (p.wdt == MLSTM_DT_F32) to_floats<float, V>(load_vec<float, V>(static_cast<const float*>(p.weight) + at), w);
+    else if (p.wdt == MLSTM_DT_F16) to_floats<__half, V>(load_vec<__half, V>(static_cast<const __half*>(p.weight) + at), w);
+    else to_floats<__nv_bfloat16, V>(load_vec<__nv_bfloat16, V>(static_cast<const __nv_bfloat16*>(p.weight) + at), w);
 }
 
-// Sum of a pair over the threads of a row: a warp, or the whole block.  Every thread gets it.
+// Sum of a pair over the threads of a row: `tpr` lanes of a warp, or the whole block.  Every thread gets it.
 template <bool WARP>
-__device__ __forceinline__ float2 row_sum(float2 v, float2* sm) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+__device__ __forceinline__ float2 row_sum(float2 v, float2* sm, int tpr) {
+    for (int o = WARP ? tpr >> 1 : 16; o > 0; o >>= 1) {
         v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
         v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
@@ -120,46 +71,46 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rms_fwd_kernel(const RmsArgs
     extern __shared__ unsigned amax[];      // QUANT: largest magnitude of every block of the row (as bits: NaN above all)
     grid_dep_wait();
     grid_dep_launch();
-    const int tpr = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const long long row = WARP ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= p.rows) return;              // (a whole warp, or never)
+    const int tpr = WARP ? p.lanes : blockDim.x, tid = WARP ? threadIdx.x & (tpr - 1) : threadIdx.x;
+    const int slot = WARP ? static_cast<int>(threadIdx.x) / tpr : 0;
+    const long long row = WARP ? static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + slot : blockIdx.x;
+    const int D = row < p.rows ? p.D : 0;   // (lanes of a warp without a row take part in its sums with nothing)
     const T* x = static_cast<const T*>(p.x) + row * p.D;
     const S* res = p.residual ? static_cast<const S*>(p.residual) + row * p.D : nullptr;
     float v[K][V];
-    RVecA<T, V> xv[K];
-    RVecA<S, V> rv[K];
+    Vec<T, V> xv[K];
+    Vec<S, V> rv[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const int e = (k * tpr + tid) * V;
-        if (e < p.D) {
-            xv[k].load(x + e);
-            if (res) rv[k].load(res + e);
+        if (e < D) {
+            xv[k] = load_vec<T, V>(x + e);
+            if (res) rv[k] = load_vec<S, V>(res + e);
         }
     }
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const int e = (k * tpr + tid) * V;
-        if (e < p.D) {
+        if (e < D) {
+            to_floats<T, V>(xv[k], v[k]);
             if (res) {
+                float r[V];
+                to_floats<S, V>(rv[k], r);
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    rv[k].v[j] = from_f32<S>(to_f32<T>(xv[k].v[j]) + to_f32<S>(rv[k].v[j]));
-                    v[k][j] = to_f32<S>(rv[k].v[j]);
-                }
-                rv[k].store(static_cast<S*>(p.sum) + row * p.D + e);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) v[k][j] = to_f32<T>(xv[k].v[j]);
+                for (int j = 0; j < V; j++) v[k][j] += r[j];
+                const Vec<S, V> t = from_floats<S, V>(v[k]);
+                store_vec<S, V>(static_cast<S*>(p.sum) + row * p.D + e, t);
+                to_floats<S, V>(t, v[k]);
             }
 #pragma unroll
             for (int j = 0; j < V; j++) acc.x = fmaf(v[k][j], v[k][j], acc.x);
         }
     }
-    acc = row_sum<WARP>(acc, sm);
+    acc = row_sum<WARP>(acc, sm, tpr);
     const float r = rsqrtf(acc.x * p.inv_d + p.eps);
     const long long wrow = p.groups > 1 ? (row / p.inner) % p.groups * p.D : 0;
-    unsigned* top = amax + (WARP ? (threadIdx.x >> 5) : 0) * (p.D / p.block);
+    unsigned* top = amax + slot * (p.D / p.block);
     if (QUANT) {
         for (int i = tid; i < p.D / p.block; i += tpr) top[i] = 0u;
         if (WARP) __syncwarp();
@@ -169,38 +120,38 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rms_fwd_kernel(const RmsArgs
     for (int k = 0; k < K; k++) {
         const int e = (k * tpr + tid) * V;
         float w[V];
-        if (e < p.D) {
+        if (e < D) {
             load_weight<V>(p, wrow + e, w);
 #pragma unroll
             for (int j = 0; j < V; j++) v[k][j] = v[k][j] * r * w[j];
         }
         if (!QUANT) {
-            if (e < p.D) store_any<V>(p.y, p.ydt, row * p.D + e, v[k]);
+            if (e < D) store_any<V>(p.y, p.ydt, row * p.D + e, v[k]);
         } else {
             unsigned m = 0u;
-            if (e < p.D) {
+            if (e < D) {
 #pragma unroll
                 for (int j = 0; j < V; j++) m = max(m, __float_as_uint(v[k][j]) & 0x7fffffffu);
             }
             // neighbouring threads of one block of values first (all of a warp's are in one block or every few are)
-            const int same = min(32, p.block / V > 0 ? p.block / V : 1);
-            if (same == 32 || (same & (same - 1)) == 0)
+            const int same = min(tpr < 32 ? tpr : 32, p.block / V > 0 ? p.block / V : 1);
+            if ((same & (same - 1)) == 0)
                 for (int o = same >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (e < p.D) atomicMax(&top[e / p.block], m);       // (the largest: no order to depend on)
+            if (e < D) atomicMax(&top[e / p.block], m);       // (the largest: no order to depend on)
         }
     }
     if (QUANT) {
         if (WARP) __syncwarp();
         else __syncthreads();
         const int blocks = p.D / p.block;
-        for (int i = tid; i < blocks; i += tpr) {
+        for (int i = tid; i < blocks && D > 0; i += tpr) {
             const float s = top[i] == 0u ? 1.0f : __fdiv_rn(__uint_as_float(top[i]), 448.0f);
             p.scale[row * blocks + i] = s;
         }
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int e = (k * tpr + tid) * V;
-            if (e < p.D) {
+            if (e < D) {
                 const unsigned t = top[e / p.block];
                 const float inv = t == 0u ? 1.0f : __fdiv_rn(448.0f, __uint_as_float(t));
                 uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.D + e;
@@ -218,16 +169,29 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rms_fwd_kernel(const RmsArgs
     }
 }
 
-// S: the stream's type, T: dy's.  Blocks (or warps) walk over the rows of one group and keep their part of the weight's gradient.
+__device__ __forceinline__ void copy16(void* shared, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(shared))), "l"(global) : "memory");
+}
+
+// S: the stream's type, T: dy's.  Blocks (or parts of warps) walk over the rows of one group and keep their part of the weight's
+// gradient.  Where a thread has eight values of a row (PIPE), its pieces of the next rows are on their way to shared memory
+// while it works on one (each thread reads back what it asked for itself: no barrier).
 template <typename T, typename S, int V, int K, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512) rms_bwd_kernel(const RmsArgs p) {
+struct RmsPipe {
+    static constexpr bool ON = V == 8 && K == 1;
+    static constexpr int STAGES = 3, NS = sizeof(S) * V / 16, NT = sizeof(T) * V / 16, PIECES = 2 * NS + NT;   // s, ds, dy in 16 bytes
+    __host__ __device__ static constexpr size_t bytes(int threads) { return ON ? static_cast<size_t>(STAGES) * PIECES * threads * 16 : 0; }
+};
+template <typename T, typename S, int V, int K, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 4 : V == 8 && K == 1 ? 2 : 1) rms_bwd_kernel(const RmsArgs p) {
+    using Pipe = RmsPipe<T, S, V, K, WARP>;
     __shared__ float2 sm[32];
-    extern __shared__ unsigned dyn[];
+    extern __shared__ __align__(16) unsigned char dyn[];
     grid_dep_wait();
     grid_dep_launch();
-    const int tpr = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const int rpb = WARP ? blockDim.x >> 5 : 1, slot = WARP ? threadIdx.x >> 5 : 0, g = blockIdx.y;
-    const long long rows_g = p.rows / p.groups;
+    const int tpr = WARP ? p.lanes : blockDim.x, tid = WARP ? threadIdx.x & (tpr - 1) : threadIdx.x;
+    const int rpb = WARP ? static_cast<int>(blockDim.x) / tpr : 1, slot = WARP ? static_cast<int>(threadIdx.x) / tpr : 0, g = blockIdx.y;
+    const long long rows_g = p.rows / p.groups, step = static_cast<long long>(gridDim.x) * rpb;
     float dw[K][V], w[K][V];
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -236,62 +200,103 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rms_bwd_kernel(const RmsArgs
         for (int j = 0; j < V; j++) dw[k][j] = 0.f;
         if (e < p.D) load_weight<V>(p, static_cast<long long>(g) * p.D + e, w[k]);
     }
-    for (long long i = static_cast<long long>(blockIdx.x) * rpb + slot; i < rows_g; i += static_cast<long long>(gridDim.x) * rpb) {
-        const long long row = p.groups > 1 ? ((i / p.inner) * p.groups + g) * p.inner + i % p.inner : i;
+    auto row_of = [&](long long i) { return p.groups > 1 ? ((i / p.inner) * p.groups + g) * p.inner + i % p.inner : i; };
+    [[maybe_unused]] uint4* ring = reinterpret_cast<uint4*>(dyn) + threadIdx.x;        // [stage][piece][thread]
+    [[maybe_unused]] const int pitch = blockDim.x;
+    auto fetch = [&](long long i, int stage) {
+        if constexpr (Pipe::ON) {
+            if (i < rows_g && tid * V < p.D) {
+                const long long at = row_of(i) * p.D + tid * V;
+                uint4* q = ring + stage * Pipe::PIECES * pitch;
+#pragma unroll
+                for (int c = 0; c < Pipe::NS; c++) {
+                    copy16(q + c * pitch, reinterpret_cast<const uint4*>(static_cast<const S*>(p.x) + at) + c);
+                    if (p.ds) copy16(q + (Pipe::NS + c) * pitch, reinterpret_cast<const uint4*>(static_cast<const S*>(p.ds) + at) + c);
+                }
+#pragma unroll
+                for (int c = 0; c < Pipe::NT; c++)
+                    copy16(q + (2 * Pipe::NS + c) * pitch, reinterpret_cast<const uint4*>(static_cast<const T*>(p.dy) + at) + c);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+    int stage = 0;
+    const long long first = static_cast<long long>(blockIdx.x) * rpb + slot;
+#pragma unroll
+    for (int k = 0; k < Pipe::STAGES - 1; k++) fetch(first + k * step, k);
+    // (the same number of turns for all lanes of a warp; a lane past the last row takes part in the sums with nothing)
+    for (long long i = first; i - slot < rows_g; i += step) {
+        const int D = i < rows_g ? p.D : 0;
+        const long long row = D ? row_of(i) : 0;
         const S* s = static_cast<const S*>(p.x) + row * p.D;
         const T* dy = static_cast<const T*>(p.dy) + row * p.D;
         const S* ds = p.ds ? static_cast<const S*>(p.ds) + row * p.D : nullptr;
-        RVecA<S, V> sv[K], dsv[K];
-        RVecA<T, V> dv[K];
+        Vec<S, V> sv[K], dsv[K];
+        Vec<T, V> dv[K];
+        if constexpr (Pipe::ON) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(Pipe::STAGES - 2) : "memory");
+            const uint4* q = ring + stage * Pipe::PIECES * pitch;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int e = (k * tpr + tid) * V;
-            if (e < p.D) {
-                sv[k].load(s + e);
-                dv[k].load(dy + e);
-                if (ds) dsv[k].load(ds + e);
+            for (int c = 0; c < Pipe::NS; c++) {
+                reinterpret_cast<uint4*>(&sv[0])[c] = q[c * pitch];
+                if (ds) reinterpret_cast<uint4*>(&dsv[0])[c] = q[(Pipe::NS + c) * pitch];
+            }
+#pragma unroll
+            for (int c = 0; c < Pipe::NT; c++) reinterpret_cast<uint4*>(&dv[0])[c] = q[(2 * Pipe::NS + c) * pitch];
+            const int into = stage == 0 ? Pipe::STAGES - 1 : stage - 1;      // used up one turn ago
+            fetch(i + (Pipe::STAGES - 1) * step, into);
+            stage = stage + 1 == Pipe::STAGES ? 0 : stage + 1;
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int e = (k * tpr + tid) * V;
+                if (e < D) {
+                    sv[k] = load_vec<S, V>(s + e);
+                    dv[k] = load_vec<T, V>(dy + e);
+                    if (ds) dsv[k] = load_vec<S, V>(ds + e);
+                }
             }
         }
         float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            if ((k * tpr + tid) * V < p.D) {
+            if ((k * tpr + tid) * V < D) {
+                float a[V], d[V];
+                to_floats<S, V>(sv[k], a);
+                to_floats<T, V>(dv[k], d);
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    const float a = to_f32<S>(sv[k].v[j]);
-                    acc.x = fmaf(a, a, acc.x);
-                    acc.y = fmaf(a * w[k][j], to_f32<T>(dv[k].v[j]), acc.y);
+                    acc.x = fmaf(a[j], a[j], acc.x);
+                    acc.y = fmaf(a[j] * w[k][j], d[j], acc.y);
                 }
             }
         }
-        acc = row_sum<WARP>(acc, sm);
+        acc = row_sum<WARP>(acc, sm, tpr);
         const float r = rsqrtf(acc.x * p.inv_d + p.eps), m = acc.y * p.inv_d * r * r;
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int e = (k * tpr + tid) * V;
-            if (e < p.D) {
-                float out[V];
+            if (e < D) {
+                float a[V], d[V], o[V];
+                to_floats<S, V>(sv[k], a);
+                to_floats<T, V>(dv[k], d);
+                if (ds) to_floats<S, V>(dsv[k], o);
+                const float m2 = -m * r;                 // r (d w - a m) + ds
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    const float a = to_f32<S>(sv[k].v[j]), d = to_f32<T>(dv[k].v[j]);
-                    out[j] = r * (d * w[k][j] - a * m);
-                    if (ds) out[j] += to_f32<S>(dsv[k].v[j]);
-                    dw[k][j] = fmaf(d * r, a, dw[k][j]);
+                    d[j] *= r;
+                    o[j] = fmaf(d[j], w[k][j], ds ? fmaf(a[j], m2, o[j]) : a[j] * m2);
+                    dw[k][j] = fmaf(d[j], a[j], dw[k][j]);
                 }
-                store_any<V>(p.dx, p.xdt, row * p.D + e, out);
-                if (p.dres) {
-                    RVecA<S, V> o;
-#pragma unroll
-                    for (int j = 0; j < V; j++) o.v[j] = from_f32<S>(out[j]);
-                    o.store(static_cast<S*>(p.dres) + row * p.D + e);
-                }
+                store_any<V>(p.dx, p.xdt, row * p.D + e, o);
+                if (p.dres) store_vec<S, V>(static_cast<S*>(p.dres) + row * p.D + e, from_floats<S, V>(o));
             }
         }
     }
     if (!p.part) return;
     float* part = p.part + (static_cast<long long>(blockIdx.x) * p.groups + g) * p.D;
-    float* sum = reinterpret_cast<float*>(dyn);
-    for (int turn = 0; turn < rpb; turn++) {        // a block's warps, one after the other
+    float* sum = reinterpret_cast<float*>(dyn + Pipe::bytes(blockDim.x));
+    for (int turn = 0; turn < rpb; turn++) {        // a block's rows at a time, one after the other
         if (WARP && turn > 0) __syncthreads();
         if (slot == turn) {
 #pragma unroll
@@ -318,27 +323,28 @@ struct RmsWeightOut {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 constexpr int RMS_MAX_D = 16384;
-// How a row is laid over threads: V values each, K times, by a warp (WARP) or a block of `threads`.
+// How a row is laid over threads: V values each, K times, by `lanes` lanes of a warp (several rows in a block of 128 threads) or, lanes
+// = 0, by a whole block of `threads`.
 struct RmsPlan {
-    int V, K, threads;
-    bool warp;
+    int V, K, threads, lanes;
+    int rows() const { return lanes ? threads / lanes : 1; }
 };
-RmsPlan rms_plan(int D, bool wide) {
-    if (!wide) {
-        if (D <= 512) return {1, 16, 128, true};
-        int t = 64;
-        while (t * 16 < D && t < 512) t *= 2;
-        return {1, t * 16 < D ? 32 : 16, t, false};
+RmsPlan rms_plan(int D, bool wide, bool bwd) {
+    const int V = wide ? 8 : 1, K = wide ? (bwd ? 1 : 2) : 16;       // the backward holds three rows and two more of floats
+    const int in_warp = wide ? (bwd ? 256 : 1024) : 512;
+    if (D <= in_warp) {
+        const int k = wide ? (D <= 256 ? 1 : D <= 512 ? 2 : 4) : K;
+        int lanes = 32;
+        while (wide && lanes > 8 && lanes / 2 * V >= D) lanes /= 2;
+        return {V, k, 128, lanes};
     }
-    if (D <= 256) return {8, 1, 128, true};
-    if (D <= 512) return {8, 2, 128, true};
-    if (D <= 1024) return {8, 4, 128, true};
-    int t = 64;
-    while (t * 16 < D && t < 512) t *= 2;
-    return {8, t * 16 < D ? 4 : 2, t, false};
+    RmsPlan p{V, K, 64, 0};
+    while (p.threads * V * p.K < D && p.threads < 512) p.threads *= 2;
+    while (p.threads * V * p.K < D) p.K *= 2;
+    return p;
 }
 int rms_bwd_blocks(long long rows_g, int groups, const RmsPlan& pl) {
-    const int rpb = pl.warp ? 4 : 1, per_sm = pl.warp ? 8 : pl.threads <= 256 ? 6 : 3;
+    const int rpb = pl.rows(), per_sm = pl.lanes ? 6 : 1024 / pl.threads;
     long long want = 148LL * per_sm / groups;
     if (want < 1) want = 1;
     const long long most = (rows_g + rpb - 1) / rpb;
@@ -346,38 +352,44 @@ int rms_bwd_blocks(long long rows_g, int groups, const RmsPlan& pl) {
 }
 
 template <typename T, typename S, bool QUANT>
-cudaError_t launch_rms_fwd(const RmsArgs& a, bool wide, cudaStream_t st) {
-    const RmsPlan pl = rms_plan(a.D, wide);
-    const int rpb = pl.warp ? 4 : 1;
+cudaError_t launch_rms_fwd(RmsArgs a, bool wide, cudaStream_t st) {
+    const RmsPlan pl = rms_plan(a.D, wide, false);
+    const int rpb = pl.rows();
+    a.lanes = pl.lanes;
     const dim3 grid(static_cast<unsigned>((a.rows + rpb - 1) / rpb)), block(pl.threads);
     const size_t smem = QUANT ? static_cast<size_t>(rpb) * (a.D / a.block) * 4 : 0;
     if (pl.V == 1) {
-        if (pl.warp) return launch_plain(rms_fwd_kernel<T, S, 1, 16, true, QUANT>, grid, block, smem, st, a);
+        if (pl.lanes) return launch_plain(rms_fwd_kernel<T, S, 1, 16, true, QUANT>, grid, block, smem, st, a);
         if (pl.K == 16) return launch_plain(rms_fwd_kernel<T, S, 1, 16, false, QUANT>, grid, block, smem, st, a);
         return launch_plain(rms_fwd_kernel<T, S, 1, 32, false, QUANT>, grid, block, smem, st, a);
     }
-    if (!pl.warp && pl.K == 4) return launch_plain(rms_fwd_kernel<T, S, 8, 4, false, QUANT>, grid, block, smem, st, a);
-    if (!pl.warp) return launch_plain(rms_fwd_kernel<T, S, 8, 2, false, QUANT>, grid, block, smem, st, a);
+    if (!pl.lanes && pl.K == 4) return launch_plain(rms_fwd_kernel<T, S, 8, 4, false, QUANT>, grid, block, smem, st, a);
+    if (!pl.lanes) return launch_plain(rms_fwd_kernel<T, S, 8, 2, false, QUANT>, grid, block, smem, st, a);
     if (pl.K == 1) return launch_plain(rms_fwd_kernel<T, S, 8, 1, true, QUANT>, grid, block, smem, st, a);
     if (pl.K == 2) return launch_plain(rms_fwd_kernel<T, S, 8, 2, true, QUANT>, grid, block, smem, st, a);
     return launch_plain(rms_fwd_kernel<T, S, 8, 4, true, QUANT>, grid, block, smem, st, a);
 }
-template <typename T, typename S>
-cudaError_t launch_rms_bwd(const RmsArgs& a, bool wide, cudaStream_t st) {
-    const RmsPlan pl = rms_plan(a.D, wide);
+template <typename T, typename S, int V, int K, bool WARP>
+cudaError_t launch_rms_bwd_k(const RmsArgs& a, const RmsPlan& pl, cudaStream_t st) {
     const dim3 grid(rms_bwd_blocks(a.rows / a.groups, a.groups, pl), a.groups), block(pl.threads);
-    const size_t smem = pl.warp && a.part ? static_cast<size_t>(a.D) * 4 : 0;
-    cudaError_t ce;
+    const size_t smem = RmsPipe<T, S, V, K, WARP>::bytes(pl.threads) + (WARP && a.part ? static_cast<size_t>(a.D) * 4 : 0);
+    auto kern = rms_bwd_kernel<T, S, V, K, WARP>;
+    if (smem > 48 * 1024) {
+        const cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (ce != cudaSuccess) return ce;
+    }
+    return launch_plain(kern, grid, block, smem, st, a);
+}
+template <typename T, typename S>
+cudaError_t launch_rms_bwd(RmsArgs a, bool wide, cudaStream_t st) {
+    const RmsPlan pl = rms_plan(a.D, wide, true);
+    a.lanes = pl.lanes;
     if (pl.V == 1)
-        ce = pl.warp ? launch_plain(rms_bwd_kernel<T, S, 1, 16, true>, grid, block, smem, st, a)
-             : pl.K == 16 ? launch_plain(rms_bwd_kernel<T, S, 1, 16, false>, grid, block, smem, st, a)
-                          : launch_plain(rms_bwd_kernel<T, S, 1, 32, false>, grid, block, smem, st, a);
-    else if (!pl.warp && pl.K == 4) ce = launch_plain(rms_bwd_kernel<T, S, 8, 4, false>, grid, block, smem, st, a);
-    else if (!pl.warp) ce = launch_plain(rms_bwd_kernel<T, S, 8, 2, false>, grid, block, smem, st, a);
-    else if (pl.K == 1) ce = launch_plain(rms_bwd_kernel<T, S, 8, 1, true>, grid, block, smem, st, a);
-    else if (pl.K == 2) ce = launch_plain(rms_bwd_kernel<T, S, 8, 2, true>, grid, block, smem, st, a);
-    else ce = launch_plain(rms_bwd_kernel<T, S, 8, 4, true>, grid, block, smem, st, a);
-    return ce;
+        return pl.lanes ? launch_rms_bwd_k<T, S, 1, 16, true>(a, pl, st)
+               : pl.K == 16 ? launch_rms_bwd_k<T, S, 1, 16, false>(a, pl, st) : launch_rms_bwd_k<T, S, 1, 32, false>(a, pl, st);
+    if (pl.lanes) return launch_rms_bwd_k<T, S, 8, 1, true>(a, pl, st);
+    return pl.K == 1 ? launch_rms_bwd_k<T, S, 8, 1, false>(a, pl, st)
+           : pl.K == 2 ? launch_rms_bwd_k<T, S, 8, 2, false>(a, pl, st) : launch_rms_bwd_k<T, S, 8, 4, false>(a, pl, st);
 }
 
 inline int elem_size(int dt) { return dt == MLSTM_DT_F32 ? 4 : 2; }
@@ -439,7 +451,7 @@ int mlstm_rms_fwd(const void* x, const void* residual, const void* weight, void*
 size_t mlstm_rms_bwd_workspace(long long rows, int D, int groups, int inner) {
     if (rms_check(rows, D, groups, inner, 0, 0, 0, false) != MLSTM_OK) return 0;
     const long long rows_g = rows / groups;
-    const int a = rms_bwd_blocks(rows_g, groups, rms_plan(D, true)), b = rms_bwd_blocks(rows_g, groups, rms_plan(D, false));
+    const int a = rms_bwd_blocks(rows_g, groups, rms_plan(D, true, true)), b = rms_bwd_blocks(rows_g, groups, rms_plan(D, false, true));
     return static_cast<size_t>(a > b ? a : b) * groups * D * sizeof(float);
 }
 
@@ -468,7 +480,7 @@ int mlstm_rms_bwd(const void* dy, const void* ds, const void* s, const void* wei
     else if (dy_dtype == MLSTM_DT_F16) ce = s_dtype == MLSTM_DT_F32 ? launch_rms_bwd<__half, float>(a, wide, st) : launch_rms_bwd<__half, __half>(a, wide, st);
     else ce = s_dtype == MLSTM_DT_F32 ? launch_rms_bwd<__nv_bfloat16, float>(a, wide, st) : launch_rms_bwd<__nv_bfloat16, __nv_bfloat16>(a, wide, st);
     if (ce == cudaSuccess && weight) {
-        const int blocks = rms_bwd_blocks(rows / groups, groups, rms_plan(D, wide));
+        const int blocks = rms_bwd_blocks(rows / groups, groups, rms_plan(D, wide, true));
         ce = launch_reduce_rows(a.part, blocks, static_cast<long long>(groups) * D, RmsWeightOut{{dweight, w_dtype}}, st);
     }
     if (ce != cudaSuccess) cudaGetLastError();

@@ -14,7 +14,7 @@
 #include <initializer_list>
 #include <type_traits>
 
-#include "mlstm_common.cuh"
+#include "pair_math.cuh"
 
 namespace mlstm {
 
@@ -43,38 +43,6 @@ struct SsmArgs {
 };
 
 __host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// ---- two floats as one operand (the packed fp32 instructions of sm_100)
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pack2(float a, float b) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(f2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    f2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f2 exp2_2(f2 x) {
-    const float2 v = unpack2(x);
-    return pack2(fast_exp2(v.x), fast_exp2(v.y));
-}
 
 // ---- loads and stores of a pair of neighbouring channels; `pairs`: aligned for one access; n: how many of the two exist
 template <typename T>
