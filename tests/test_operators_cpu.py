@@ -95,8 +95,8 @@ def test_scratch_sizes(pkg):
     # the channels alone fill the chip: one pass, no scratch; a narrow, long call is cut into segments
     assert L.mlstm_ssm_fwd_workspace(8, 4096, 4096, 1, 16) == 0 < L.mlstm_ssm_fwd_workspace(1, 16384, 512, 1, 16)
     assert L.mlstm_ssm_fwd_workspace(1, 16384, 512, 1, 65) == 0 == L.mlstm_ssm_bwd_workspace(1, 16384, 512, 3, 16)
-    # a state of every 32 positions, the channels of each group rounded up to 64
-    assert L.mlstm_ssm_checkpoint_floats(2, 100, 96, 2, 16) == 2 * 4 * 16 * 128
+    # a state of every 16 positions, the channels of each group rounded up to 64
+    assert L.mlstm_ssm_checkpoint_floats(2, 100, 96, 2, 16) == 2 * 7 * 16 * 128
     # partial dB, dC: at most 512 MB at a time, whatever the batch
     one = 64 * 4096 * 16 * 8
     for B in (1, 4, 64, 1000):

@@ -41,6 +41,7 @@ __device__ __forceinline__ float rcp_f(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp_f(1.0f + fast_exp2(x * -1.44269504088896340736f)); }
 // sigmoid of both: two hardware functions each, good to a few units in the last place (exp(-x) = inf gives 0)
 __device__ __forceinline__ f2 sigmoid2(f2 x) {
     const float2 e = unpack2(exp2_2(mul2(x, pack2(-1.44269504088896340736f, -1.44269504088896340736f))));

@@ -5,9 +5,7 @@
 namespace mlstm {
 namespace {
 
-// positions staged in shared memory at a time (with eight warps half as many: what they hand over fits the 48 KB of a plain launch)
-template <int W>
-constexpr int SSM_TILE = W == 8 ? 8 : 16;
+constexpr int SSM_TILE = 16;        // positions handed over at a time
 
 struct SsmFwdArgs : SsmArgs {
     const float* initial;           // [Bt, Ch, N] or nullptr
@@ -15,40 +13,122 @@ struct SsmFwdArgs : SsmArgs {
     float* state_out;               // [Bt, Ch, N] or nullptr
 };
 
-template <int K, int W>
+template <int K>
 struct SsmFwdSmem {
-    float4 dl[SSM_TILE<W>][32];                    // delta, delta x of the lane's two channels
-    float4 bc[SSM_TILE<W>][K * W];                 // B, B, C, C
-    float2 y[W][SSM_TILE<W>][32];                  // every warp's part of the output
+    float4 dl[2][SSM_TILE][32];                         // delta, delta x of the lane's two channels
+    float4 bc[2][SSM_TILE][K * SSM_WARPS];              // B, B, C, C
+    float2 y[2][SSM_WARPS][SSM_TILE][32];               // every warp's part of the output
 };
+// barriers, one for each buffer
+enum : int { BAR_FULL = 1, BAR_EMPTY = 3, BAR_Y_FULL = 5, BAR_Y_EMPTY = 7 };
 
 // One CTA: 64 channels, one segment.  OUT: outputs (and the states that are kept); else only what the segment adds to the state.
-template <typename T, int K, int W, bool OUT>
-__global__ void __launch_bounds__(32 * W) ssm_fwd_kernel(const SsmFwdArgs p) {
-    constexpr int TILE = SSM_TILE<W>, NP = K * W, IT = TILE / W, BI = (TILE * NP + 32 * W - 1) / (32 * W);
-    __shared__ SsmFwdSmem<K, W> sm;
+// Tile i uses buffer i & 1 of everything.  A buffer's first use waits for nothing, and what the last two uses leave is not
+// announced, so every barrier is met exactly as often by either half.
+template <typename T, int K, bool OUT, bool PAIRS>
+__global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArgs p) {
+    constexpr int TILE = SSM_TILE, W = SSM_WARPS, NP = K * W;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    SsmFwdSmem<K>& sm = *reinterpret_cast<SsmFwdSmem<K>*>(smem_raw);
     grid_dep_wait();
     grid_dep_launch();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, seg = blockIdx.y;
+    const int lane = threadIdx.x & 31, b = blockIdx.z, seg = blockIdx.y;
     const SsmTile ch = ssm_tile(p, blockIdx.x, lane);
-    const int t_begin = seg * p.seglen, t_end = min(p.S, t_begin + p.seglen);
-    const bool pairs = p.pairs != 0;
+    const int t_begin = seg * p.seglen, t_end = min(p.S, t_begin + p.seglen), tiles = ceil_div(t_end - t_begin, TILE);
 
-    const T* xp = static_cast<const T*>(p.x) + b * p.sx.b + ch.c;
-    const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt.b + ch.c;
-    const T* zp = p.z ? static_cast<const T*>(p.z) + b * p.sz.b + ch.c : nullptr;
-    const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + static_cast<long long>(ch.g) * p.N;
-    const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + static_cast<long long>(ch.g) * p.N;
+    if (threadIdx.x >= 32 * W) {
+        constexpr int AW = SSM_AIDES, AT = 32 * AW, IT = TILE / AW, BI = (TILE * NP + AT - 1) / AT, BSTEP = AT / NP;
+        static_assert(TILE % AW == 0 && AT % NP == 0 && BI * BSTEP >= TILE, "every value of a tile has a thread");
+        const bool gated = OUT && p.z;
+        const int tid = threadIdx.x - 32 * W, warp = tid >> 5;
+        // rows of this thread: t0 + warp + AW i; positions and state of its B, C: t0 + bt + BSTEP i, bn
+        const T* xp = static_cast<const T*>(p.x) + b * p.sx.b + (t_begin + warp) * p.sx.t + ch.c;
+        const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt.b + (t_begin + warp) * p.sdt.t + ch.c;
+        const T* zp = gated ? static_cast<const T*>(p.z) + b * p.sz.b + (t_begin + warp) * p.sz.t + ch.c : nullptr;
+        T* yp = OUT ? static_cast<T*>(p.y) + (static_cast<size_t>(b) * p.S + t_begin + warp) * p.Ch + ch.c : nullptr;
+        const int bt = tid / NP, bn = tid % NP;
+        const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + (t_begin + bt) * p.sB.t + static_cast<long long>(ch.g) * p.N + bn;
+        const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + (t_begin + bt) * p.sC.t + static_cast<long long>(ch.g) * p.N + bn;
+        const f2 bias = param2(p.bias, ch.c, ch.n), skip = OUT ? param2(p.D, ch.c, ch.n) : 0;
+        Raw2<T> rx[IT], rdt[IT], rz[IT];
+        T rB[BI], rC[BI];
+        auto fetch = [&](int left) {            // left: positions of the segment from the tile on
+#pragma unroll
+            for (int i = 0; i < IT; i++) {
+                const int n = warp + AW * i < left ? ch.n : 0;
+                rx[i] = load_raw2<PAIRS>(xp + (AW * i) * p.sx.t, n);
+                rdt[i] = load_raw2<PAIRS>(dtp + (AW * i) * p.sdt.t, n);
+                if (gated) rz[i] = load_raw2<PAIRS>(zp + (AW * i) * p.sz.t, n);
+            }
+            xp += TILE * p.sx.t;
+            dtp += TILE * p.sdt.t;
+            if (gated) zp += TILE * p.sz.t;
+#pragma unroll
+            for (int i = 0; i < BI; i++) {
+                const bool in = bn < p.N && bt + BSTEP * i < min(left, TILE);
+                rB[i] = in ? Bp[(BSTEP * i) * p.sB.t] : from_f32<T>(0.f);
+                if (OUT) rC[i] = in ? Cp[(BSTEP * i) * p.sC.t] : from_f32<T>(0.f);
+            }
+            Bp += TILE * p.sB.t;
+            Cp += TILE * p.sC.t;
+        };
+        f2 part[IT], gate[IT], next_part[IT], next_gate[IT];     // D x and silu(z) of the positions that this thread finishes
+        auto stage = [&](int tile) {                             // (the tile has been fetched)
+            const int buf = tile & 1, left = t_end - t_begin - tile * TILE;
+            if (tile >= 2) half_sync<SSM_THREADS>(BAR_EMPTY + buf);
+#pragma unroll
+            for (int i = 0; i < IT; i++) {
+                const int r = warp + AW * i;
+                const float2 x = to_float2<T>(rx[i]);
+                f2 d = delta2(to_float2<T>(rdt[i]), bias, p.softplus);
+                if (r >= left) d = 0;           // a step of 0 leaves the state
+                const f2 xv = pack2(x.x, x.y);
+                *reinterpret_cast<ulonglong2*>(&sm.dl[buf][r][lane]) = make_ulonglong2(d, mul2(d, xv));
+                if (OUT) next_part[i] = p.D ? mul2(skip, xv) : 0;
+                if (gated) {
+                    const float2 z = to_float2<T>(rz[i]);
+                    next_gate[i] = mul2(pack2(z.x, z.y), sigmoid2(pack2(z.x, z.y)));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < BI; i++) {
+                const float bv = to_f32<T>(rB[i]), cv = OUT ? to_f32<T>(rC[i]) : 0.f;
+                if (bt + BSTEP * i < TILE) sm.bc[buf][bt + BSTEP * i][bn] = make_float4(bv, bv, cv, cv);
+            }
+            half_arrive<SSM_THREADS>(BAR_FULL + buf);
+            if (left > TILE) fetch(left - TILE);
+        };
+        fetch(t_end - t_begin);
+        stage(0);
+        for (int tile = 0; tile < tiles; tile++) {
+            if (OUT) {
+#pragma unroll
+                for (int i = 0; i < IT; i++) {
+                    part[i] = next_part[i];
+                    if (gated) gate[i] = next_gate[i];
+                }
+            }
+            if (tile + 1 < tiles) stage(tile + 1);
+            if (OUT) {
+                const int buf = tile & 1, left = t_end - t_begin - tile * TILE;
+                half_sync<SSM_THREADS>(BAR_Y_FULL + buf);
+#pragma unroll
+                for (int i = 0; i < IT; i++) {
+                    const int r = warp + AW * i;
+                    f2 v = part[i];
+#pragma unroll
+                    for (int w = 0; w < W; w++) v = add2(v, *reinterpret_cast<const f2*>(&sm.y[buf][w][r][lane]));
+                    if (gated) v = mul2(v, gate[i]);
+                    if (r < left) store_pair<PAIRS>(yp + static_cast<size_t>(AW * i) * p.Ch, unpack2(v), ch.n);
+                }
+                yp += static_cast<size_t>(TILE) * p.Ch;
+                if (tile + 2 < tiles) half_arrive<SSM_THREADS>(BAR_Y_EMPTY + buf);
+            }
+        }
+        return;
+    }
 
-    float2 bias = make_float2(0.f, 0.f), skip = make_float2(0.f, 0.f);
-    if (p.bias) {
-        if (ch.n > 0) bias.x = p.bias[ch.c];
-        if (ch.n > 1) bias.y = p.bias[ch.c + 1];
-    }
-    if (OUT && p.D) {
-        if (ch.n > 0) skip.x = p.D[ch.c];
-        if (ch.n > 1) skip.y = p.D[ch.c + 1];
-    }
+    const int warp = threadIdx.x >> 5;
     f2 rate[K], h[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -69,12 +149,12 @@ __global__ void __launch_bounds__(32 * W) ssm_fwd_kernel(const SsmFwdArgs p) {
         rate[k] = pack2(r0, r1);
         h[k] = pack2(h0, h1);
     }
+    auto seg_state = [&](int j, int n) { return p.seg_end + ((static_cast<size_t>(b) * p.nseg + j) * p.N + n) * p.Cpad + ch.cp; };
     if (!OUT && seg == 0) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int n = warp * K + k;
-            if (n < p.N)
-                *reinterpret_cast<f2*>(p.seg_end + ((static_cast<size_t>(b) * p.nseg + p.nseg - 1) * p.N + n) * p.Cpad + ch.cp) = h[k];
+            if (n < p.N) *reinterpret_cast<f2*>(seg_state(p.nseg - 1, n)) = h[k];
             h[k] = 0;
         }
     }
@@ -82,79 +162,37 @@ __global__ void __launch_bounds__(32 * W) ssm_fwd_kernel(const SsmFwdArgs p) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int n = warp * K + k;
-            if (n < p.N)
-                h[k] = *reinterpret_cast<const f2*>(p.seg_end + ((static_cast<size_t>(b) * p.nseg + p.nseg - 1) * p.N + n) * p.Cpad + ch.cp);
+            if (n < p.N) h[k] = *reinterpret_cast<const f2*>(seg_state(p.nseg - 1, n));
         }
         for (int j = 0; j < seg; j++) {
-            const size_t sj = (static_cast<size_t>(b) * p.nseg + j);
-            const f2 sum = *reinterpret_cast<const f2*>(p.seg_sum + sj * p.Cpad + ch.cp);
+            const f2 sum = *reinterpret_cast<const f2*>(p.seg_sum + (static_cast<size_t>(b) * p.nseg + j) * p.Cpad + ch.cp);
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
-                if (n < p.N)
-                    h[k] = fma2(exp2_2(mul2(sum, rate[k])), h[k],
-                                *reinterpret_cast<const f2*>(p.seg_end + (sj * p.N + n) * p.Cpad + ch.cp));
+                if (n < p.N) h[k] = fma2(exp2_2(mul2(sum, rate[k])), h[k], *reinterpret_cast<const f2*>(seg_state(j, n)));
             }
         }
     }
-
-    Raw2<T> rx[IT], rdt[IT], rz[IT];
-    T rB[BI], rC[BI];
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < IT; i++) {
-            const int t = t0 + warp + W * i, n = t < t_end ? ch.n : 0;
-            rx[i] = load_raw2<T>(xp + t * p.sx.t, pairs, n);
-            rdt[i] = load_raw2<T>(dtp + t * p.sdt.t, pairs, n);
-            if (OUT && zp) rz[i] = load_raw2<T>(zp + t * p.sz.t, pairs, n);
-        }
-#pragma unroll
-        for (int i = 0; i < BI; i++) {
-            const int e = threadIdx.x + i * 32 * W, t = t0 + e / NP, n = e % NP;
-            const bool in = e < TILE * NP && n < p.N && t < t_end;
-            rB[i] = in ? Bp[t * p.sB.t + n] : from_f32<T>(0.f);
-            if (OUT) rC[i] = in ? Cp[t * p.sC.t + n] : from_f32<T>(0.f);
-        }
-    };
     [[maybe_unused]] f2 sum = 0;
-    fetch(t_begin);
-    for (int t0 = t_begin; t0 < t_end; t0 += TILE) {
-        [[maybe_unused]] float2 x[IT], z[IT];
-#pragma unroll
-        for (int i = 0; i < IT; i++) {
-            const int r = warp + W * i;
-            x[i] = to_float2<T>(rx[i]);
-            if (OUT && zp) z[i] = to_float2<T>(rz[i]);
-            float2 d = to_float2<T>(rdt[i]);
-            d.x += bias.x;
-            d.y += bias.y;
-            if (p.softplus) d = make_float2(softplus_f(d.x), softplus_f(d.y));
-            if (t0 + r >= t_end) d = make_float2(0.f, 0.f);     // a step of 0 leaves the state
-            sm.dl[r][lane] = make_float4(d.x, d.y, d.x * x[i].x, d.y * x[i].y);
-        }
-#pragma unroll
-        for (int i = 0; i < BI; i++) {
-            const int e = threadIdx.x + i * 32 * W;
-            const float bv = to_f32<T>(rB[i]), cv = OUT ? to_f32<T>(rC[i]) : 0.f;
-            if (e < TILE * NP) sm.bc[e / NP][e % NP] = make_float4(bv, bv, cv, cv);
-        }
-        __syncthreads();
-        if (t0 + TILE < t_end) fetch(t0 + TILE);
-        if (OUT && p.ckpt && t0 % SSM_CK == 0) {
-            const size_t row = static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + t0 / SSM_CK;
+    for (int tile = 0; tile < tiles; tile++) {
+        const int buf = tile & 1;
+        if (OUT && p.ckpt && tile % (SSM_CK / TILE) == 0) {
+            const size_t row = static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + (t_begin + tile * TILE) / SSM_CK;
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
                 if (n < p.N) *reinterpret_cast<f2*>(p.ckpt + (row * p.N + n) * p.Cpad + ch.cp) = h[k];
             }
         }
+        half_sync<SSM_THREADS>(BAR_FULL + buf);
+        if (OUT && tile >= 2) half_sync<SSM_THREADS>(BAR_Y_EMPTY + buf);
 #pragma unroll 1
         for (int half = 0; half < TILE; half += SSM_ROWS) {
             f2 dl[SSM_ROWS], dx[SSM_ROWS];
             [[maybe_unused]] f2 y[SSM_ROWS];
 #pragma unroll
             for (int r = 0; r < SSM_ROWS; r++) {
-                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[half + r][lane]);
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[buf][half + r][lane]);
                 dl[r] = v.x;
                 dx[r] = v.y;
                 if (OUT) y[r] = 0;
@@ -166,7 +204,7 @@ __global__ void __launch_bounds__(32 * W) ssm_fwd_kernel(const SsmFwdArgs p) {
                 f2 s = h[k];
 #pragma unroll
                 for (int r = 0; r < SSM_ROWS; r++) {
-                    const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&sm.bc[half + r][warp * K + k]);
+                    const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&sm.bc[buf][half + r][warp * K + k]);
                     s = fma2(exp2_2(mul2(dl[r], rate[k])), s, mul2(dx[r], bc.x));
                     if (OUT) y[r] = fma2(s, bc.y, y[r]);
                 }
@@ -174,37 +212,19 @@ __global__ void __launch_bounds__(32 * W) ssm_fwd_kernel(const SsmFwdArgs p) {
             }
             if (OUT) {
 #pragma unroll
-                for (int r = 0; r < SSM_ROWS; r++) *reinterpret_cast<f2*>(&sm.y[warp][half + r][lane]) = y[r];
+                for (int r = 0; r < SSM_ROWS; r++) *reinterpret_cast<f2*>(&sm.y[buf][warp][half + r][lane]) = y[r];
             }
         }
-        __syncthreads();
-        if (OUT) {
-#pragma unroll
-            for (int i = 0; i < IT; i++) {
-                const int r = warp + W * i;
-                if (t0 + r < t_end) {
-                    float2 v = make_float2(skip.x * x[i].x, skip.y * x[i].y);
-                    if (!p.D) v = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        const float2 part = sm.y[w][r][lane];
-                        v.x += part.x;
-                        v.y += part.y;
-                    }
-                    if (zp) v = make_float2(v.x * silu_f(z[i].x), v.y * silu_f(z[i].y));
-                    store_pair<T>(static_cast<T*>(p.y) + (static_cast<size_t>(b) * p.S + t0 + r) * p.Ch + ch.c, v, pairs, ch.n);
-                }
-            }
-        }
+        if (OUT) half_arrive<SSM_THREADS>(BAR_Y_FULL + buf);
+        if (tile + 2 < tiles) half_arrive<SSM_THREADS>(BAR_EMPTY + buf);
     }
     if (!OUT) {
-        const size_t sj = static_cast<size_t>(b) * p.nseg + seg;
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int n = warp * K + k;
-            if (n < p.N) *reinterpret_cast<f2*>(p.seg_end + (sj * p.N + n) * p.Cpad + ch.cp) = h[k];
+            if (n < p.N) *reinterpret_cast<f2*>(seg_state(seg, n)) = h[k];
         }
-        if (warp == 0) *reinterpret_cast<f2*>(p.seg_sum + sj * p.Cpad + ch.cp) = sum;
+        if (warp == 0) *reinterpret_cast<f2*>(p.seg_sum + (static_cast<size_t>(b) * p.nseg + seg) * p.Cpad + ch.cp) = sum;
     } else if (p.state_out && seg == p.nseg - 1) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -219,22 +239,29 @@ __global__ void __launch_bounds__(32 * W) ssm_fwd_kernel(const SsmFwdArgs p) {
     }
 }
 
-template <typename T, int K, int W>
+template <typename T, int K, bool OUT>
+cudaError_t launch_ssm_fwd_pass(const SsmFwdArgs& a, int segs, cudaStream_t st) {
+    auto kern = a.pairs ? ssm_fwd_kernel<T, K, OUT, true> : ssm_fwd_kernel<T, K, OUT, false>;
+    constexpr size_t smem = sizeof(SsmFwdSmem<K>);
+    const cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (ce != cudaSuccess) return ce;
+    return launch_plain(kern, dim3(static_cast<unsigned>(a.G * a.tiles_g), segs, a.Bt), dim3(SSM_THREADS), smem, st, a);
+}
+template <typename T, int K>
 cudaError_t launch_ssm_fwd(const SsmFwdArgs& a, cudaStream_t st) {
-    const unsigned tiles = static_cast<unsigned>(a.G * a.tiles_g);
     if (a.nseg > 1) {
-        const cudaError_t ce = launch_plain(ssm_fwd_kernel<T, K, W, false>, dim3(tiles, a.nseg - 1, a.Bt), dim3(32 * W), 0, st, a);
+        const cudaError_t ce = launch_ssm_fwd_pass<T, K, false>(a, a.nseg - 1, st);
         if (ce != cudaSuccess) return ce;
     }
-    return launch_plain(ssm_fwd_kernel<T, K, W, true>, dim3(tiles, a.nseg, a.Bt), dim3(32 * W), 0, st, a);
+    return launch_ssm_fwd_pass<T, K, true>(a, a.nseg, st);
 }
 template <typename T>
 cudaError_t launch_ssm_fwd_n(const SsmFwdArgs& a, cudaStream_t st) {
-    if (a.N <= 4) return launch_ssm_fwd<T, 1, 4>(a, st);
-    if (a.N <= 8) return launch_ssm_fwd<T, 2, 4>(a, st);
-    if (a.N <= 16) return launch_ssm_fwd<T, 4, 4>(a, st);
-    if (a.N <= 32) return launch_ssm_fwd<T, 8, 4>(a, st);
-    return launch_ssm_fwd<T, 8, 8>(a, st);
+    if (a.N <= 4) return launch_ssm_fwd<T, 1>(a, st);
+    if (a.N <= 8) return launch_ssm_fwd<T, 2>(a, st);
+    if (a.N <= 16) return launch_ssm_fwd<T, 4>(a, st);
+    if (a.N <= 32) return launch_ssm_fwd<T, 8>(a, st);
+    return launch_ssm_fwd<T, 16>(a, st);
 }
 
 // ---------------------------------------------------------------------------------------------- a few new tokens
@@ -390,7 +417,7 @@ bool ssm_pairs(const SsmArgs& a, int es, std::initializer_list<const void*> more
 
 namespace {
 
-constexpr int SSM_FWD_CTAS = 4;     // CTAs of 4 warps that an SM is filled with
+constexpr int SSM_FWD_CTAS = 2;     // CTAs that an SM is filled with
 
 }  // namespace
 }  // namespace mlstm

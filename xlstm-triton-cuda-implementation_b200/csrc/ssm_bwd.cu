@@ -6,8 +6,8 @@
 //     dx_t = delta_t sum_n g_t B_t + D e_t        ddelta_t = x_t sum_n g_t B_t + sum_n A g_t u_t
 //     dz_t = dy_t (sum_n C_t h_t + D x_t) silu'(z_t),   ddt = ddelta * sigmoid(dt + bias) behind a softplus
 // The positions are walked from the last to the first in runs of SSM_CK: the states inside a run are computed again from the
-// state that the forward kept in front of it, first at every SSM_ROWS positions (to shared memory), then for one group of
-// SSM_ROWS at a time in registers, together with the exponentials that the way back needs again.
+// state that the forward kept in front of it, first the one in front of the second half, then for one half of SSM_ROWS
+// positions at a time all of them, in registers, together with the exponentials that the way back needs again.
 //
 // The sums over the channels (dB, dC) run over a CTA's 64 channels by a transposing butterfly (half of the values change hands at
 // every step, so 8 values cost 9 shuffles instead of 40) and over the CTAs of a group in a second kernel; the sums over the
@@ -27,16 +27,35 @@ struct SsmBwdArgs : SsmArgs {
 };
 
 constexpr int BWD_SUBS = SSM_CK / SSM_ROWS;
+static_assert(BWD_SUBS == 2, "the two halves of a run of positions have buffers of their own");
 
-template <int K, int W>
+template <typename T, int K, int W>
 struct SsmBwdSmem {
     float4 dl[SSM_CK][32];                  // delta, delta x
     float2 e[SSM_CK][32];                   // dy silu(z)
     float4 bc[SSM_CK][K * W];               // B, B, C, C
-    float2 h[BWD_SUBS][K * W][32];          // the states in front of every SSM_ROWS positions
-    float2 red[3][W][SSM_ROWS][32];         // every warp's sums over its states: g B, A g u, C h
-    float2 bcg[SSM_ROWS][K * W];            // dB, dC of this CTA's channels
+    float2 h[K * W][32];                    // the states in front of the second half
+    float2 red[BWD_SUBS][3][W][SSM_ROWS][32];   // every warp's sums over its states: g B, A g u, C h
+    float2 bcg[BWD_SUBS][SSM_ROWS][K * W];  // dB, dC of this CTA's channels
+    // what the next run of positions needs, on its way from memory; every thread reads back what it asked for itself
+    Raw2<T> raw[2][4][SSM_CK][32];          // x, dt, dy, z
+    float2 h0[2][K * W][32];                // the states in front of the run
 };
+
+__device__ __forceinline__ void copy_async8(void* shared, const void* global) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(shared))), "l"(global) : "memory");
+}
+// a pair of channels to shared memory: asynchronously where it is one aligned access
+template <bool PAIRS, typename T>
+__device__ __forceinline__ void copy_raw2(Raw2<T>* shared, const T* global, int n) {
+    if constexpr (PAIRS) {
+        constexpr int bytes = 2 * sizeof(T);
+        if (n) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(shared))), "l"(global), "n"(bytes) : "memory");
+        else *shared = Raw2<T>{};
+    } else {
+        *shared = load_raw2<false>(global, n);
+    }
+}
 
 // Sums 8 values over the warp; the sum of v[i] arrives in the lanes 4 i .. 4 i + 3.
 __device__ __forceinline__ float butterfly8(float (&v)[SSM_ROWS], int lane) {
@@ -53,14 +72,8 @@ __device__ __forceinline__ float butterfly8(float (&v)[SSM_ROWS], int lane) {
     return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
 }
 
-__device__ __forceinline__ float2 delta_of(float2 raw, float2 bias, int softplus) {
-    raw.x += bias.x;
-    raw.y += bias.y;
-    return softplus ? make_float2(softplus_f(raw.x), softplus_f(raw.y)) : raw;
-}
-
 // What one segment adds to the gradient of the state in front of it: G = exp(delta A) (G + C e), from the last position back.
-template <typename T, int K, int W>
+template <typename T, int K, int W, bool PAIRS>
 __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs p) {
     constexpr int TILE = SSM_ROWS, NP = K * W, IT = TILE / W, BI = (TILE * NP) / (32 * W) > 0 ? (TILE * NP) / (32 * W) : 1;
     __shared__ float4 sm_d[TILE][32];       // delta, e
@@ -70,16 +83,11 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = p.b0 + blockIdx.z, seg = blockIdx.y + 1;
     const SsmTile ch = ssm_tile(p, blockIdx.x, lane);
     const int t_begin = seg * p.seglen, t_end = min(p.S, t_begin + p.seglen);
-    const bool pairs = p.pairs != 0;
     const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt.b + ch.c;
     const T* zp = p.z ? static_cast<const T*>(p.z) + b * p.sz.b + ch.c : nullptr;
     const T* dyp = static_cast<const T*>(p.dy) + static_cast<size_t>(b) * p.S * p.Ch + ch.c;
     const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + static_cast<long long>(ch.g) * p.N;
-    float2 bias = make_float2(0.f, 0.f);
-    if (p.bias) {
-        if (ch.n > 0) bias.x = p.bias[ch.c];
-        if (ch.n > 1) bias.y = p.bias[ch.c + 1];
-    }
+    const f2 bias = param2(p.bias, ch.c, ch.n);
     f2 rate[K], G[K], sum = 0;
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -100,14 +108,15 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
 #pragma unroll
         for (int i = 0; i < IT; i++) {
             const int r = warp + W * i, t = t0 + r, n = t < t_end ? ch.n : 0;
-            float2 d = delta_of(to_float2<T>(load_raw2<T>(dtp + t * p.sdt.t, pairs, n)), bias, p.softplus);
-            float2 e = to_float2<T>(load_raw2<T>(dyp + static_cast<size_t>(t) * p.Ch, pairs, n));
+            f2 d = delta2(to_float2<T>(load_raw2<PAIRS>(dtp + t * p.sdt.t, n)), bias, p.softplus);
+            const float2 dy = to_float2<T>(load_raw2<PAIRS>(dyp + static_cast<size_t>(t) * p.Ch, n));
+            f2 e = pack2(dy.x, dy.y);
             if (zp) {
-                const float2 z = to_float2<T>(load_raw2<T>(zp + t * p.sz.t, pairs, n));
-                e = make_float2(e.x * silu_f(z.x), e.y * silu_f(z.y));
+                const float2 z = to_float2<T>(load_raw2<PAIRS>(zp + t * p.sz.t, n));
+                e = mul2(e, mul2(pack2(z.x, z.y), sigmoid2(pack2(z.x, z.y))));
             }
-            if (t >= t_end) d = make_float2(0.f, 0.f);
-            sm_d[r][lane] = make_float4(d.x, d.y, e.x, e.y);
+            if (t >= t_end) d = 0;
+            *reinterpret_cast<ulonglong2*>(&sm_d[r][lane]) = make_ulonglong2(d, e);
         }
 #pragma unroll
         for (int i = 0; i < BI; i++) {
@@ -141,35 +150,28 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
     if (warp == 0) *reinterpret_cast<f2*>(p.seg_sum + sj * p.Cpad + ch.cp) = sum;
 }
 
-template <typename T, int K, int W, bool GATED>
+template <typename T, int K, int W, bool GATED, bool PAIRS>
 __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
-    constexpr int NP = K * W, IT = SSM_ROWS / W;
+    constexpr int NP = K * W, IT = SSM_CK / W, SIT = SSM_ROWS / W, BI = SSM_CK * NP / (32 * W) > 0 ? SSM_CK * NP / (32 * W) : 1, BSTEP = 32 * W / NP;
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    SsmBwdSmem<K, W>& sm = *reinterpret_cast<SsmBwdSmem<K, W>*>(smem_raw);
+    SsmBwdSmem<T, K, W>& sm = *reinterpret_cast<SsmBwdSmem<T, K, W>*>(smem_raw);
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bl = blockIdx.z, b = p.b0 + bl, seg = blockIdx.y;
     const SsmTile ch = ssm_tile(p, blockIdx.x, lane);
     const int t_begin = seg * p.seglen, t_end = min(p.S, t_begin + p.seglen);
-    const bool pairs = p.pairs != 0;
 
     const T* xp = static_cast<const T*>(p.x) + b * p.sx.b + ch.c;
     const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt.b + ch.c;
     const T* zp = GATED ? static_cast<const T*>(p.z) + b * p.sz.b + ch.c : nullptr;
     const size_t row0 = static_cast<size_t>(b) * p.S;
     const T* dyp = static_cast<const T*>(p.dy) + row0 * p.Ch + ch.c;
-    const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + static_cast<long long>(ch.g) * p.N;
-    const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + static_cast<long long>(ch.g) * p.N;
+    const int bt = threadIdx.x / NP, bn = threadIdx.x % NP;
+    const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + static_cast<long long>(ch.g) * p.N + bn;
+    const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + static_cast<long long>(ch.g) * p.N + bn;
 
-    float2 bias = make_float2(0.f, 0.f), skip = make_float2(0.f, 0.f), dskip = make_float2(0.f, 0.f), dbias = make_float2(0.f, 0.f);
-    if (p.bias) {
-        if (ch.n > 0) bias.x = p.bias[ch.c];
-        if (ch.n > 1) bias.y = p.bias[ch.c + 1];
-    }
-    if (p.D) {
-        if (ch.n > 0) skip.x = p.D[ch.c];
-        if (ch.n > 1) skip.y = p.D[ch.c + 1];
-    }
+    const f2 bias = param2(p.bias, ch.c, ch.n), skip = param2(p.D, ch.c, ch.n);
+    f2 dskip = 0, dbias = 0;
     f2 rate[K], G[K], dA[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -195,72 +197,75 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
         }
     }
 
+    T rB[BI], rC[BI];
+    auto fetch = [&](int tc, int buf) {             // the run of positions that starts at tc
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const int r = warp + W * i, t = tc + r, n = t < t_end ? ch.n : 0;
+            copy_raw2<PAIRS>(&sm.raw[buf][0][r][lane], xp + t * p.sx.t, n);
+            copy_raw2<PAIRS>(&sm.raw[buf][1][r][lane], dtp + t * p.sdt.t, n);
+            copy_raw2<PAIRS>(&sm.raw[buf][2][r][lane], dyp + static_cast<size_t>(t) * p.Ch, n);
+            if (GATED) copy_raw2<PAIRS>(&sm.raw[buf][3][r][lane], zp + t * p.sz.t, n);
+        }
+        const size_t row = static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + tc / SSM_CK;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int n = warp * K + k;
+            if (n < p.N) copy_async8(&sm.h0[buf][n][lane], p.ckpt + (row * p.N + n) * p.Cpad + ch.cp);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < BI; i++) {
+            const int t = tc + bt + BSTEP * i;
+            const bool in = bn < p.N && bt + BSTEP * i < SSM_CK && t < t_end;
+            rB[i] = in ? Bp[t * p.sB.t] : from_f32<T>(0.f);
+            rC[i] = in ? Cp[t * p.sC.t] : from_f32<T>(0.f);
+        }
+    };
     const int chunks = ceil_div(t_end - t_begin, SSM_CK);
+    fetch(t_begin + (chunks - 1) * SSM_CK, (chunks - 1) & 1);
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
-        const int tc = t_begin + chunk * SSM_CK, subs = ceil_div(min(SSM_CK, t_end - tc), SSM_ROWS);
-        f2 h[K];
-        {
-            const size_t row = static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + tc / SSM_CK;
+        const int tc = t_begin + chunk * SSM_CK, subs = ceil_div(min(SSM_CK, t_end - tc), SSM_ROWS), buf = chunk & 1;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        // (the run behind this one has been read: its last barrier lies in front of everything that is written here)
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const int r = warp + W * i;
+            const float2 x = to_float2<T>(sm.raw[buf][0][r][lane]), dy = to_float2<T>(sm.raw[buf][2][r][lane]);
+            f2 d = delta2(to_float2<T>(sm.raw[buf][1][r][lane]), bias, p.softplus), e = pack2(dy.x, dy.y);
+            if (GATED) {
+                const float2 z = to_float2<T>(sm.raw[buf][3][r][lane]);
+                e = mul2(e, mul2(pack2(z.x, z.y), sigmoid2(pack2(z.x, z.y))));
+            }
+            if (tc + r >= t_end) d = 0;
+            *reinterpret_cast<ulonglong2*>(&sm.dl[r][lane]) = make_ulonglong2(d, mul2(d, pack2(x.x, x.y)));
+            *reinterpret_cast<f2*>(&sm.e[r][lane]) = e;
+        }
+#pragma unroll
+        for (int i = 0; i < BI; i++) {
+            const float bv = to_f32<T>(rB[i]), cv = to_f32<T>(rC[i]);
+            if (bt + BSTEP * i < SSM_CK) sm.bc[bt + BSTEP * i][bn] = make_float4(bv, bv, cv, cv);
+        }
+        __syncthreads();
+        if (chunk > 0) fetch(tc - SSM_CK, buf ^ 1);
+        if (subs > 1) {         // the states in front of the second half (each warp its own)
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
-                h[k] = n < p.N ? *reinterpret_cast<const f2*>(p.ckpt + (row * p.N + n) * p.Cpad + ch.cp) : 0;
-            }
-        }
-#pragma unroll 4
-        for (int r = warp; r < SSM_CK; r += W) {
-            const int t = tc + r, n = t < t_end ? ch.n : 0;
-            const float2 x = to_float2<T>(load_raw2<T>(xp + t * p.sx.t, pairs, n));
-            float2 d = delta_of(to_float2<T>(load_raw2<T>(dtp + t * p.sdt.t, pairs, n)), bias, p.softplus);
-            float2 e = to_float2<T>(load_raw2<T>(dyp + static_cast<size_t>(t) * p.Ch, pairs, n));
-            if (GATED) {
-                const float2 z = to_float2<T>(load_raw2<T>(zp + t * p.sz.t, pairs, n));
-                e = make_float2(e.x * silu_f(z.x), e.y * silu_f(z.y));
-            }
-            if (t >= t_end) d = make_float2(0.f, 0.f);
-            sm.dl[r][lane] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
-            sm.e[r][lane] = e;
-        }
-#pragma unroll
-        for (int i = 0; i < K; i++) {
-            const int x = threadIdx.x + i * 32 * W, t = tc + x / NP, n = x % NP;
-            const bool in = n < p.N && t < t_end;
-            const float bv = in ? to_f32<T>(Bp[t * p.sB.t + n]) : 0.f, cv = in ? to_f32<T>(Cp[t * p.sC.t + n]) : 0.f;
-            sm.bc[x / NP][n] = make_float4(bv, bv, cv, cv);
-        }
-        __syncthreads();
-        // the states in front of every SSM_ROWS positions (each warp its own)
-#pragma unroll 1
-        for (int sub = 0; sub < subs; sub++) {
-#pragma unroll
-            for (int k = 0; k < K; k++) *reinterpret_cast<f2*>(&sm.h[sub][warp * K + k][lane]) = h[k];
-            if (sub + 1 < subs) {
+                if (n >= p.N) break;
+                f2 s = *reinterpret_cast<const f2*>(&sm.h0[buf][n][lane]);
 #pragma unroll
                 for (int r = 0; r < SSM_ROWS; r++) {
-                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[sub * SSM_ROWS + r][lane]);
-#pragma unroll
-                    for (int k = 0; k < K; k++)
-                        h[k] = fma2(exp2_2(mul2(v.x, rate[k])), h[k],
-                                    mul2(v.y, *reinterpret_cast<const f2*>(&sm.bc[sub * SSM_ROWS + r][warp * K + k])));
+                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[r][lane]);
+                    s = fma2(exp2_2(mul2(v.x, rate[k])), s, mul2(v.y, *reinterpret_cast<const f2*>(&sm.bc[r][n])));
                 }
+                *reinterpret_cast<f2*>(&sm.h[n][lane]) = s;
             }
         }
 #pragma unroll 1
         for (int sub = subs - 1; sub >= 0; sub--) {
             const int q = sub * SSM_ROWS;
-            // for the positions that this thread finishes
-            Raw2<T> rx[IT], rdt[IT], rdy[IT];
-            [[maybe_unused]] Raw2<T> rz[IT];
-#pragma unroll
-            for (int i = 0; i < IT; i++) {
-                const int t = tc + q + warp + W * i, n = t < t_end ? ch.n : 0;
-                rx[i] = load_raw2<T>(xp + t * p.sx.t, pairs, n);
-                rdt[i] = load_raw2<T>(dtp + t * p.sdt.t, pairs, n);
-                if (GATED) {
-                    rz[i] = load_raw2<T>(zp + t * p.sz.t, pairs, n);
-                    rdy[i] = load_raw2<T>(dyp + static_cast<size_t>(t) * p.Ch, pairs, n);
-                }
-            }
+            const float2* front = sub ? &sm.h[0][lane] : &sm.h0[buf][0][lane];
             f2 dl[SSM_ROWS], dx[SSM_ROWS], e[SSM_ROWS], sb[SSM_ROWS], su[SSM_ROWS];
             [[maybe_unused]] f2 y[SSM_ROWS];
 #pragma unroll
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
                 if (n >= p.N) break;
-                f2 a[SSM_ROWS], u[SSM_ROWS], s = *reinterpret_cast<const f2*>(&sm.h[sub][n][lane]);
+                f2 a[SSM_ROWS], u[SSM_ROWS], s = *reinterpret_cast<const f2*>(front + n * 32);
                 float part[SSM_ROWS];
 #pragma unroll
                 for (int r = 0; r < SSM_ROWS; r++) {
@@ -305,59 +310,54 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
                 }
                 G[k] = g;
                 const float db = butterfly8(part, lane);
-                if ((lane & 3) == 0) sm.bcg[lane >> 2][n] = make_float2(db, dc);
+                if ((lane & 3) == 0) sm.bcg[sub][lane >> 2][n] = make_float2(db, dc);
             }
 #pragma unroll
             for (int r = 0; r < SSM_ROWS; r++) {
-                *reinterpret_cast<f2*>(&sm.red[0][warp][r][lane]) = sb[r];
-                *reinterpret_cast<f2*>(&sm.red[1][warp][r][lane]) = su[r];
-                if (GATED) *reinterpret_cast<f2*>(&sm.red[2][warp][r][lane]) = y[r];
+                *reinterpret_cast<f2*>(&sm.red[sub][0][warp][r][lane]) = sb[r];
+                *reinterpret_cast<f2*>(&sm.red[sub][1][warp][r][lane]) = su[r];
+                if (GATED) *reinterpret_cast<f2*>(&sm.red[sub][2][warp][r][lane]) = y[r];
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < IT; i++) {
+            for (int i = 0; i < SIT; i++) {
                 const int r = warp + W * i, t = tc + q + r;
                 if (t < t_end) {
                     f2 vs = 0, vu = 0, vy = 0;
 #pragma unroll
                     for (int w = 0; w < W; w++) {
-                        vs = add2(vs, *reinterpret_cast<const f2*>(&sm.red[0][w][r][lane]));
-                        vu = add2(vu, *reinterpret_cast<const f2*>(&sm.red[1][w][r][lane]));
-                        if (GATED) vy = add2(vy, *reinterpret_cast<const f2*>(&sm.red[2][w][r][lane]));
+                        vs = add2(vs, *reinterpret_cast<const f2*>(&sm.red[sub][0][w][r][lane]));
+                        vu = add2(vu, *reinterpret_cast<const f2*>(&sm.red[sub][1][w][r][lane]));
+                        if (GATED) vy = add2(vy, *reinterpret_cast<const f2*>(&sm.red[sub][2][w][r][lane]));
                     }
-                    const float2 s = unpack2(vs), u = unpack2(vu), x = to_float2<T>(rx[i]), ev = sm.e[q + r][lane];
-                    const float4 d = sm.dl[q + r][lane];
-                    constexpr float LN2 = 0.69314718055994530942f;      // the rates are in units of log2
-                    float2 dd = make_float2(fmaf(x.x, s.x, LN2 * u.x), fmaf(x.y, s.y, LN2 * u.y));
+                    const float2 xv = to_float2<T>(sm.raw[buf][0][q + r][lane]);
+                    const f2 x = pack2(xv.x, xv.y), ev = *reinterpret_cast<const f2*>(&sm.e[q + r][lane]);
+                    const f2 d = *reinterpret_cast<const f2*>(&sm.dl[q + r][lane]);
+                    f2 dd = fma2(x, vs, mul2(splat2(0.69314718055994530942f), vu));      // (the rates are in units of log2)
                     if (p.softplus) {
-                        const float2 raw = to_float2<T>(rdt[i]);
-                        dd.x *= sigmoid_f(raw.x + bias.x);
-                        dd.y *= sigmoid_f(raw.y + bias.y);
+                        const float2 raw = to_float2<T>(sm.raw[buf][1][q + r][lane]);
+                        dd = mul2(dd, sigmoid2(add2(pack2(raw.x, raw.y), bias)));
                     }
-                    dbias.x += dd.x;
-                    dbias.y += dd.y;
-                    dskip.x = fmaf(ev.x, x.x, dskip.x);
-                    dskip.y = fmaf(ev.y, x.y, dskip.y);
+                    dbias = add2(dbias, dd);
+                    dskip = fma2(ev, x, dskip);
                     const size_t at = (row0 + t) * p.Ch + ch.c;
-                    store_pair<T>(static_cast<T*>(p.ddt) + at, dd, pairs, ch.n);
-                    store_pair<T>(static_cast<T*>(p.dx) + at, make_float2(fmaf(d.x, s.x, p.D ? skip.x * ev.x : 0.f), fmaf(d.y, s.y, p.D ? skip.y * ev.y : 0.f)),
-                                  pairs, ch.n);
+                    store_pair<PAIRS>(static_cast<T*>(p.ddt) + at, unpack2(dd), ch.n);
+                    store_pair<PAIRS>(static_cast<T*>(p.dx) + at, unpack2(p.D ? fma2(d, vs, mul2(skip, ev)) : mul2(d, vs)), ch.n);
                     if (GATED) {
-                        const float2 z = to_float2<T>(rz[i]), dy = to_float2<T>(rdy[i]);
-                        float2 yv = unpack2(vy);
-                        if (p.D) yv = make_float2(fmaf(skip.x, x.x, yv.x), fmaf(skip.y, x.y, yv.y));
-                        const float s0 = sigmoid_f(z.x), s1 = sigmoid_f(z.y);
-                        store_pair<T>(static_cast<T*>(p.dz) + at,
-                                      make_float2(dy.x * yv.x * s0 * fmaf(z.x, 1.0f - s0, 1.0f), dy.y * yv.y * s1 * fmaf(z.y, 1.0f - s1, 1.0f)),
-                                      pairs, ch.n);
+                        const float2 zv = to_float2<T>(sm.raw[buf][3][q + r][lane]), dy = to_float2<T>(sm.raw[buf][2][q + r][lane]);
+                        if (p.D) vy = fma2(skip, x, vy);
+                        const f2 z = pack2(zv.x, zv.y), sg = sigmoid2(z);        // silu' = sg (1 + z (1 - sg))
+                        const f2 slope = mul2(sg, fma2(z, fma2(sg, splat2(-1.0f), splat2(1.0f)), splat2(1.0f)));
+                        store_pair<PAIRS>(static_cast<T*>(p.dz) + at, unpack2(mul2(pack2(dy.x, dy.y), mul2(vy, slope))), ch.n);
                     }
                 }
             }
-            for (int x = threadIdx.x; x < SSM_ROWS * p.N; x += 32 * W) {
-                const int r = x / p.N, n = x - r * p.N, t = tc + q + r;
-                if (t < t_end) p.bc_part[((static_cast<size_t>(blockIdx.x) * p.nb + bl) * p.S + t) * p.N + n] = sm.bcg[r][n];
+#pragma unroll
+            for (int i = 0; i < (SSM_ROWS * NP + 32 * W - 1) / (32 * W); i++) {
+                const int r = bt + BSTEP * i, t = tc + q + r;
+                if (r < SSM_ROWS && t < t_end && bn < p.N)
+                    p.bc_part[((static_cast<size_t>(blockIdx.x) * p.nb + bl) * p.S + t) * p.N + bn] = sm.bcg[sub][r][bn];
             }
-            __syncthreads();
         }
     }
     float* part = p.param_part + (static_cast<size_t>(b) * p.nseg + seg) * (p.N + 2) * p.Cpad + ch.cp;
@@ -366,18 +366,15 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
         const int n = warp * K + k;
         if (n < p.N) *reinterpret_cast<f2*>(part + static_cast<size_t>(n) * p.Cpad) = dA[k];
     }
-    sm.red[0][warp][0][lane] = dskip;
-    sm.red[1][warp][0][lane] = dbias;
+    __syncthreads();
+    *reinterpret_cast<f2*>(&sm.red[0][0][warp][0][lane]) = dskip;
+    *reinterpret_cast<f2*>(&sm.red[0][1][warp][0][lane]) = dbias;
     __syncthreads();
     if (warp < 2) {
-        float2 v = make_float2(0.f, 0.f);
+        f2 v = 0;
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float2 q = sm.red[warp][w][0][lane];
-            v.x += q.x;
-            v.y += q.y;
-        }
-        *reinterpret_cast<float2*>(part + static_cast<size_t>(p.N + warp) * p.Cpad) = v;
+        for (int w = 0; w < W; w++) v = add2(v, *reinterpret_cast<const f2*>(&sm.red[0][warp][w][0][lane]));
+        *reinterpret_cast<f2*>(part + static_cast<size_t>(p.N + warp) * p.Cpad) = v;
     }
 }
 
@@ -418,7 +415,7 @@ struct SsmParamOut {
 };
 
 constexpr size_t SSM_BWD_PART_MAX = 512u << 20;     // bytes of dB, dC partials in scratch at one time (at least one batch entry)
-constexpr int SSM_BWD_CTAS = 3;                     // CTAs of 4 warps that an SM is filled with
+constexpr int SSM_BWD_CTAS = 2;                     // CTAs that an SM is filled with
 
 struct SsmBwdWs {
     float *seg_end, *seg_sum, *param;
@@ -453,13 +450,14 @@ SsmBwdWs ssm_bwd_carve(void* ws, const SsmArgs& a) {
 template <typename T, int K, int W>
 cudaError_t launch_ssm_bwd(SsmBwdArgs a, const SsmBwdWs& w, void* dB, void* dC, cudaStream_t st) {
     const unsigned tiles = static_cast<unsigned>(a.G * a.tiles_g);
-    constexpr size_t smem = sizeof(SsmBwdSmem<K, W>);
-    auto kern = a.z ? ssm_bwd_kernel<T, K, W, true> : ssm_bwd_kernel<T, K, W, false>;
+    constexpr size_t smem = sizeof(SsmBwdSmem<T, K, W>);
+    auto kern = a.z ? (a.pairs ? ssm_bwd_kernel<T, K, W, true, true> : ssm_bwd_kernel<T, K, W, true, false>)
+                     : (a.pairs ? ssm_bwd_kernel<T, K, W, false, true> : ssm_bwd_kernel<T, K, W, false, false>);
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     for (int b0 = 0; b0 < a.Bt && ce == cudaSuccess; b0 += w.nb) {
         a.b0 = b0;
         a.nb = a.Bt - b0 < w.nb ? a.Bt - b0 : w.nb;
-        if (a.nseg > 1) ce = launch_plain(ssm_back_state_kernel<T, K, W>, dim3(tiles, a.nseg - 1, a.nb), dim3(32 * W), 0, st, a);
+        if (a.nseg > 1) ce = launch_plain(a.pairs ? ssm_back_state_kernel<T, K, W, true> : ssm_back_state_kernel<T, K, W, false>, dim3(tiles, a.nseg - 1, a.nb), dim3(32 * W), 0, st, a);
         if (ce == cudaSuccess) ce = launch_plain(kern, dim3(tiles, a.nseg, a.nb), dim3(32 * W), smem, st, a);
         const long long rows = static_cast<long long>(a.nb) * a.S;
         if (ce == cudaSuccess)

@@ -7,9 +7,11 @@
 // Everything between the loads and the stores is fp32.
 //
 // Layout of the work: a CTA owns SSM_CH = 64 neighbouring channels of one group, a lane two of them, so that a position's
-// row of 16-bit values is one 128-byte access and every arithmetic instruction is one on a pair of floats (f32x2); the warps of
-// the CTA share the N states among them, K each.  B_t[n] and C_t[n] are the same for all channels of a CTA: they lie in shared
-// memory twice each, as pairs, and come as one 16-byte broadcast.
+// row of 16-bit values is one 128-byte access and every arithmetic instruction is one on a pair of floats (f32x2).  Four of its
+// warps do the recurrence, K of the N states each; four more prepare what these read (delta and delta x of 64 channels, and
+// B_t[n], C_t[n], which are the same for all channels, twice each as pairs for one 16-byte broadcast) and finish what they
+// leave (the sum over the states, D x, the gate).  The two halves work on different tiles of positions at the same time, two
+// buffers each way, handed over by named barriers.
 #pragma once
 #include <initializer_list>
 #include <type_traits>
@@ -21,7 +23,10 @@ namespace mlstm {
 constexpr int SSM_CH = 64;          // channels per CTA
 constexpr int SSM_ROWS = 8;         // positions whose operands a warp holds in registers at a time
 constexpr int SSM_MAX_N = 64;       // states per channel
-constexpr int SSM_CK = 32;          // positions between two states that the forward keeps for the backward
+constexpr int SSM_WARPS = 4;        // warps that do the recurrence
+constexpr int SSM_AIDES = 4;       // warps that prepare and finish
+constexpr int SSM_THREADS = 32 * (SSM_WARPS + SSM_AIDES);
+constexpr int SSM_CK = 16;          // positions between two states that the forward keeps for the backward
 
 // strides in elements between batch entries and between positions; the last dimension is contiguous
 struct SsmStrides {
@@ -44,30 +49,30 @@ struct SsmArgs {
 
 __host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// ---- loads and stores of a pair of neighbouring channels; `pairs`: aligned for one access; n: how many of the two exist
+// ---- barriers between the two halves of a block: COUNT threads in all, of which some only announce themselves (arrive)
+template <int COUNT>
+__device__ __forceinline__ void half_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(COUNT) : "memory"); }
+template <int COUNT>
+__device__ __forceinline__ void half_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(COUNT) : "memory"); }
+
+// ---- loads and stores of a pair of neighbouring channels; PAIRS: aligned for one access; n: how many of the two exist
 template <typename T>
 struct Raw2 { uint32_t v; };
 template <>
 struct Raw2<float> { float2 v; };
 
-template <typename T>
-__device__ __forceinline__ Raw2<T> load_raw2(const T* p, bool pairs, int n) {
+template <bool PAIRS, typename T>
+__device__ __forceinline__ Raw2<T> load_raw2(const T* p, int n) {
     Raw2<T> r;
-    if constexpr (sizeof(T) == 4) {
-        r.v = make_float2(0.f, 0.f);
-        if (n == 2 && pairs) r.v = *reinterpret_cast<const float2*>(p);
-        else {
-            if (n > 0) r.v.x = p[0];
-            if (n > 1) r.v.y = p[1];
-        }
+    if constexpr (PAIRS) {                  // (n is 0 or 2)
+        if constexpr (sizeof(T) == 4) r.v = make_float2(0.f, 0.f);
+        else r.v = 0u;
+        if (n) r.v = *reinterpret_cast<const decltype(r.v)*>(p);
+    } else if constexpr (sizeof(T) == 4) {
+        r.v = make_float2(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f);
     } else {
-        r.v = 0u;
-        if (n == 2 && pairs) r.v = *reinterpret_cast<const uint32_t*>(p);
-        else {
-            const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-            if (n > 0) r.v = q[0];
-            if (n > 1) r.v |= static_cast<uint32_t>(q[1]) << 16;
-        }
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+        r.v = (n > 0 ? q[0] : 0u) | (n > 1 ? static_cast<uint32_t>(q[1]) << 16 : 0u);
     }
     return r;
 }
@@ -77,9 +82,10 @@ __device__ __forceinline__ float2 to_float2(Raw2<T> r) {
     else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&r.v));
     else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.v));
 }
-template <typename T>
-__device__ __forceinline__ void store_pair(T* p, float2 v, bool pairs, int n) {
-    if (n == 2 && pairs) {
+template <bool PAIRS, typename T>
+__device__ __forceinline__ void store_pair(T* p, float2 v, int n) {
+    if constexpr (PAIRS) {
+        if (n == 0) return;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = v;
         else if constexpr (std::is_same_v<T, __half>) *reinterpret_cast<__half2*>(p) = __float22half2_rn(v);
         else *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v);
@@ -89,25 +95,36 @@ __device__ __forceinline__ void store_pair(T* p, float2 v, bool pairs, int n) {
     }
 }
 
-// log(1 + e) for 0 <= e <= 1 by the series of 2 atanh(e / (2 + e)): s = e / (2 + e) <= 1/3, and the first term left out is
-// below 2e-8 of the sum.  (1 + e rounds away what a small e has.)
-__device__ __forceinline__ float log1p_unit(float e) {
-    const float s = __fdividef(e, 2.0f + e), t = s * s;
-    float p = fmaf(t, 1.0f / 13.0f, 1.0f / 11.0f);
-    p = fmaf(t, p, 1.0f / 9.0f);
-    p = fmaf(t, p, 1.0f / 7.0f);
-    p = fmaf(t, p, 1.0f / 5.0f);
-    p = fmaf(t, p, 1.0f / 3.0f);
-    return 2.0f * fmaf(s * t, p, s);
+// softplus of both: max(v, 0) + log(1 + e), e = exp(-|v|).  The logarithm of 1 + e, which rounds away what a small e has, is taken
+// by the series of 2 atanh(s), s = e / (2 + e) <= 1/3; the first term left out is below 2e-8 of the sum.
+__device__ __forceinline__ f2 splat2(float a) { return pack2(a, a); }
+__device__ __forceinline__ f2 softplus2(float2 v) {
+    const f2 e = exp2_2(mul2(pack2(fabsf(v.x), fabsf(v.y)), splat2(-1.44269504088896340736f)));
+    const float2 d = unpack2(add2(e, splat2(2.0f)));
+    const f2 s = mul2(e, pack2(rcp_f(d.x), rcp_f(d.y))), t = mul2(s, s);
+    f2 q = fma2(t, splat2(2.0f / 13.0f), splat2(2.0f / 11.0f));
+    q = fma2(t, q, splat2(2.0f / 9.0f));
+    q = fma2(t, q, splat2(2.0f / 7.0f));
+    q = fma2(t, q, splat2(2.0f / 5.0f));
+    q = fma2(t, q, splat2(2.0f / 3.0f));
+    q = fma2(t, q, splat2(2.0f));
+    return fma2(s, q, pack2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
 }
-__device__ __forceinline__ float softplus_f(float v) { return fmaxf(v, 0.0f) + log1p_unit(__expf(-fabsf(v))); }
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float softplus_f(float v) { return unpack2(softplus2(make_float2(v, v))).x; }
+// delta of both channels from the pre-activation
+__device__ __forceinline__ f2 delta2(float2 raw, f2 bias, int softplus) {
+    const f2 v = add2(pack2(raw.x, raw.y), bias);
+    return softplus ? softplus2(unpack2(v)) : v;
+}
 
 // A in units of log2; -inf as the lowest finite value, so that a step of 0 leaves the state (0 * -inf would be NaN)
 __device__ __forceinline__ float decay_rate(float a) {
     const float r = a * 1.44269504088896340736f;
     return r < -3.0e38f ? -3.0e38f : r;
 }
+
+// values of a parameter of the lane's two channels
+__device__ __forceinline__ f2 param2(const float* p, int c, int n) { return pack2(p && n > 0 ? p[c] : 0.f, p && n > 1 ? p[c + 1] : 0.f); }
 
 // Where a CTA's channels lie: group, first channel, channels of this lane (0, 1 or 2).
 struct SsmTile {

@@ -16,8 +16,8 @@ D, dt_bias: [channels], float32; N <= 64.  D, z and dt_bias may be None.  y has 
 buffer).  Up to 8 positions take a kernel for decoding, as ``mlstm_chunkwise`` does for its mixer.  A position with delta = 0
 (no ``dt_softplus``) leaves the state as it is: so a batch of different lengths is padded on the left.
 
-Inputs that require gradients get them (no states in that case): the forward then keeps the state in front of every 32
-positions (N / 8 float32 values per element of x) and the backward recomputes what lies between.
+Inputs that require gradients get them (no states in that case): the forward then keeps the state in front of every 16
+positions (N / 16 float32 values per element of x) and the backward recomputes what lies between.
 The reference has no such operator; its own mixer with the same interface to states is ``mlstm_scan``.
 """
 import ctypes
