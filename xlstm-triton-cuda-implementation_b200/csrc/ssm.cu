@@ -25,7 +25,7 @@ enum : int { BAR_FULL = 1, BAR_EMPTY = 3, BAR_Y_FULL = 5, BAR_Y_EMPTY = 7 };
 // One CTA: 64 channels, one segment.  OUT: outputs (and the states that are kept); else only what the segment adds to the state.
 // Tile i uses buffer i & 1 of everything.  A buffer's first use waits for nothing, and what the last two uses leave is not
 // announced, so every barrier is met exactly as often by either half.
-template <typename T, int K, bool OUT, bool PAIRS>
+template <typename T, int K, bool OUT, bool PAIRS, bool FULL>
 __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArgs p) {
     constexpr int TILE = SSM_TILE, W = SSM_WARPS, NP = K * W;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArg
             }
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                if (warp * K + k >= p.N) break;         // (the same for the whole warp)
+                if (!FULL && warp * K + k >= p.N) break;        // (FULL: N = 4 K.  A branch here would keep the states' chains apart)
                 f2 s = h[k];
 #pragma unroll
                 for (int r = 0; r < SSM_ROWS; r++) {
@@ -241,7 +241,8 @@ __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArg
 
 template <typename T, int K, bool OUT>
 cudaError_t launch_ssm_fwd_pass(const SsmFwdArgs& a, int segs, cudaStream_t st) {
-    auto kern = a.pairs ? ssm_fwd_kernel<T, K, OUT, true> : ssm_fwd_kernel<T, K, OUT, false>;
+    auto kern = a.pairs && a.N == K * SSM_WARPS ? ssm_fwd_kernel<T, K, OUT, true, true>
+                : a.pairs ? ssm_fwd_kernel<T, K, OUT, true, false> : ssm_fwd_kernel<T, K, OUT, false, false>;
     constexpr size_t smem = sizeof(SsmFwdSmem<K>);
     const cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (ce != cudaSuccess) return ce;

@@ -26,17 +26,20 @@ struct SsmBwdArgs : SsmArgs {
     int b0, nb;                     // batches of this launch: b0 .. b0 + nb - 1
 };
 
-constexpr int BWD_SUBS = SSM_CK / SSM_ROWS;
-static_assert(BWD_SUBS == 2, "the two halves of a run of positions have buffers of their own");
+#ifndef BR
+#define BR 8
+#endif
+constexpr int BWD_ROWS = BR;                            // positions whose states are held in registers at a time
+constexpr int BWD_SUBS = SSM_CK / BWD_ROWS;
 
 template <typename T, int K, int W>
 struct SsmBwdSmem {
     float4 dl[SSM_CK][32];                  // delta, delta x
     float2 e[SSM_CK][32];                   // dy silu(z)
     float4 bc[SSM_CK][K * W];               // B, B, C, C
-    float2 h[K * W][32];                    // the states in front of the second half
-    float2 red[BWD_SUBS][3][W][SSM_ROWS][32];   // every warp's sums over its states: g B, A g u, C h
-    float2 bcg[BWD_SUBS][SSM_ROWS][K * W];  // dB, dC of this CTA's channels
+    float2 h[BWD_SUBS - 1][K * W][32];      // the states in front of every BWD_ROWS positions but the first
+    float2 red[2][3][W][BWD_ROWS][32];      // every warp's sums over its states: g B, A g u, C h
+    float2 bcg[2][BWD_ROWS][K * W];         // dB, dC of this CTA's channels
     // what the next run of positions needs, on its way from memory; every thread reads back what it asked for itself
     Raw2<T> raw[2][4][SSM_CK][32];          // x, dt, dy, z
     float2 h0[2][K * W][32];                // the states in front of the run
@@ -57,19 +60,27 @@ __device__ __forceinline__ void copy_raw2(Raw2<T>* shared, const T* global, int 
     }
 }
 
-// Sums 8 values over the warp; the sum of v[i] arrives in the lanes 4 i .. 4 i + 3.
-__device__ __forceinline__ float butterfly8(float (&v)[SSM_ROWS], int lane) {
+// Sums R values of two kinds over the warp; those of position i arrive in lane 32 / R * i (and in the lanes up to the next).  The two
+// are independent: the latency of one hides the other's.
+template <int R>
+__device__ __forceinline__ float2 butterfly(float (&v)[R], float (&w)[R], int lane) {
 #pragma unroll
-    for (int half = 4, o = 16; half > 0; half >>= 1, o >>= 1) {
+    for (int half = R / 2, o = 16; half > 0; half >>= 1, o >>= 1) {
         const bool up = (lane & o) != 0;
 #pragma unroll
         for (int i = 0; i < half; i++) {
-            const float keep = up ? v[i + half] : v[i], send = up ? v[i] : v[i + half];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+            const float kv = up ? v[i + half] : v[i], sv = up ? v[i] : v[i + half];
+            const float kw = up ? w[i + half] : w[i], sw = up ? w[i] : w[i + half];
+            v[i] = kv + __shfl_xor_sync(0xffffffffu, sv, o);
+            w[i] = kw + __shfl_xor_sync(0xffffffffu, sw, o);
         }
     }
-    v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
-    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+#pragma unroll
+    for (int o = 16 / R; o > 0; o >>= 1) {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        w[0] += __shfl_xor_sync(0xffffffffu, w[0], o);
+    }
+    return make_float2(v[0], w[0]);
 }
 
 // What one segment adds to the gradient of the state in front of it: G = exp(delta A) (G + C e), from the last position back.
@@ -150,9 +161,9 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
     if (warp == 0) *reinterpret_cast<f2*>(p.seg_sum + sj * p.Cpad + ch.cp) = sum;
 }
 
-template <typename T, int K, int W, bool GATED, bool PAIRS>
+template <typename T, int K, int W, bool GATED, bool PAIRS, bool FULL>
 __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
-    constexpr int NP = K * W, IT = SSM_CK / W, SIT = SSM_ROWS / W, BI = SSM_CK * NP / (32 * W) > 0 ? SSM_CK * NP / (32 * W) : 1, BSTEP = 32 * W / NP;
+    constexpr int NP = K * W, IT = SSM_CK / W, SIT = BWD_ROWS / W > 0 ? BWD_ROWS / W : 1, BI = SSM_CK * NP / (32 * W) > 0 ? SSM_CK * NP / (32 * W) : 1, BSTEP = 32 * W / NP;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SsmBwdSmem<T, K, W>& sm = *reinterpret_cast<SsmBwdSmem<T, K, W>*>(smem_raw);
     grid_dep_wait();
@@ -161,14 +172,17 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
     const SsmTile ch = ssm_tile(p, blockIdx.x, lane);
     const int t_begin = seg * p.seglen, t_end = min(p.S, t_begin + p.seglen);
 
-    const T* xp = static_cast<const T*>(p.x) + b * p.sx.b + ch.c;
-    const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt.b + ch.c;
-    const T* zp = GATED ? static_cast<const T*>(p.z) + b * p.sz.b + ch.c : nullptr;
+    const int chunks = ceil_div(t_end - t_begin, SSM_CK), t_last = t_begin + (chunks - 1) * SSM_CK;
+    // rows of this thread in the run that is fetched next (the last one first): tc + warp + W i
+    const T* xp = static_cast<const T*>(p.x) + b * p.sx.b + (t_last + warp) * p.sx.t + ch.c;
+    const T* dtp = static_cast<const T*>(p.dt) + b * p.sdt.b + (t_last + warp) * p.sdt.t + ch.c;
+    const T* zp = GATED ? static_cast<const T*>(p.z) + b * p.sz.b + (t_last + warp) * p.sz.t + ch.c : nullptr;
     const size_t row0 = static_cast<size_t>(b) * p.S;
-    const T* dyp = static_cast<const T*>(p.dy) + row0 * p.Ch + ch.c;
+    const T* dyp = static_cast<const T*>(p.dy) + (row0 + t_last + warp) * p.Ch + ch.c;
     const int bt = threadIdx.x / NP, bn = threadIdx.x % NP;
-    const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + static_cast<long long>(ch.g) * p.N + bn;
-    const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + static_cast<long long>(ch.g) * p.N + bn;
+    const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + (t_last + bt) * p.sB.t + static_cast<long long>(ch.g) * p.N + bn;
+    const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + (t_last + bt) * p.sC.t + static_cast<long long>(ch.g) * p.N + bn;
+    const float* kept = p.ckpt + ((static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + t_last / SSM_CK) * p.N + warp * K) * p.Cpad + ch.cp;
 
     const f2 bias = param2(p.bias, ch.c, ch.n), skip = param2(p.D, ch.c, ch.n);
     f2 dskip = 0, dbias = 0;
@@ -198,34 +212,36 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
     }
 
     T rB[BI], rC[BI];
-    auto fetch = [&](int tc, int buf) {             // the run of positions that starts at tc
+    auto fetch = [&](int left, int buf) {           // left: positions of the segment from the run on
 #pragma unroll
         for (int i = 0; i < IT; i++) {
-            const int r = warp + W * i, t = tc + r, n = t < t_end ? ch.n : 0;
-            copy_raw2<PAIRS>(&sm.raw[buf][0][r][lane], xp + t * p.sx.t, n);
-            copy_raw2<PAIRS>(&sm.raw[buf][1][r][lane], dtp + t * p.sdt.t, n);
-            copy_raw2<PAIRS>(&sm.raw[buf][2][r][lane], dyp + static_cast<size_t>(t) * p.Ch, n);
-            if (GATED) copy_raw2<PAIRS>(&sm.raw[buf][3][r][lane], zp + t * p.sz.t, n);
+            const int r = warp + W * i, n = r < left ? ch.n : 0;
+            copy_raw2<PAIRS>(&sm.raw[buf][0][r][lane], xp + (W * i) * p.sx.t, n);
+            copy_raw2<PAIRS>(&sm.raw[buf][1][r][lane], dtp + (W * i) * p.sdt.t, n);
+            copy_raw2<PAIRS>(&sm.raw[buf][2][r][lane], dyp + static_cast<size_t>(W * i) * p.Ch, n);
+            if (GATED) copy_raw2<PAIRS>(&sm.raw[buf][3][r][lane], zp + (W * i) * p.sz.t, n);
         }
-        const size_t row = static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + tc / SSM_CK;
+        xp -= SSM_CK * p.sx.t;
+        dtp -= SSM_CK * p.sdt.t;
+        dyp -= static_cast<size_t>(SSM_CK) * p.Ch;
+        if (GATED) zp -= SSM_CK * p.sz.t;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int n = warp * K + k;
-            if (n < p.N) copy_async8(&sm.h0[buf][n][lane], p.ckpt + (row * p.N + n) * p.Cpad + ch.cp);
-        }
+        for (int k = 0; k < K; k++)
+            if (warp * K + k < p.N) copy_async8(&sm.h0[buf][warp * K + k][lane], kept + static_cast<size_t>(k) * p.Cpad);
+        kept -= static_cast<size_t>(p.N) * p.Cpad;
         asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < BI; i++) {
-            const int t = tc + bt + BSTEP * i;
-            const bool in = bn < p.N && bt + BSTEP * i < SSM_CK && t < t_end;
-            rB[i] = in ? Bp[t * p.sB.t] : from_f32<T>(0.f);
-            rC[i] = in ? Cp[t * p.sC.t] : from_f32<T>(0.f);
+            const bool in = bn < p.N && bt + BSTEP * i < min(left, SSM_CK);
+            rB[i] = in ? Bp[(BSTEP * i) * p.sB.t] : from_f32<T>(0.f);
+            rC[i] = in ? Cp[(BSTEP * i) * p.sC.t] : from_f32<T>(0.f);
         }
+        Bp -= SSM_CK * p.sB.t;
+        Cp -= SSM_CK * p.sC.t;
     };
-    const int chunks = ceil_div(t_end - t_begin, SSM_CK);
-    fetch(t_begin + (chunks - 1) * SSM_CK, (chunks - 1) & 1);
+    fetch(t_end - t_last, (chunks - 1) & 1);
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
-        const int tc = t_begin + chunk * SSM_CK, subs = ceil_div(min(SSM_CK, t_end - tc), SSM_ROWS), buf = chunk & 1;
+        const int tc = t_begin + chunk * SSM_CK, subs = ceil_div(min(SSM_CK, t_end - tc), BWD_ROWS), buf = chunk & 1;
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         // (the run behind this one has been read: its last barrier lies in front of everything that is written here)
 #pragma unroll
@@ -247,29 +263,34 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
             if (bt + BSTEP * i < SSM_CK) sm.bc[bt + BSTEP * i][bn] = make_float4(bv, bv, cv, cv);
         }
         __syncthreads();
-        if (chunk > 0) fetch(tc - SSM_CK, buf ^ 1);
-        if (subs > 1) {         // the states in front of the second half (each warp its own)
+        if (chunk > 0) fetch(SSM_CK, buf ^ 1);
+        // the states in front of every BWD_ROWS positions (each warp its own)
+        if (subs > 1) {
+            f2 s[K];
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-                const int n = warp * K + k;
-                if (n >= p.N) break;
-                f2 s = *reinterpret_cast<const f2*>(&sm.h0[buf][n][lane]);
+            for (int k = 0; k < K; k++) s[k] = *reinterpret_cast<const f2*>(&sm.h0[buf][warp * K + k][lane]);
+#pragma unroll 1
+            for (int sub = 1; sub < subs; sub++) {
 #pragma unroll
-                for (int r = 0; r < SSM_ROWS; r++) {
-                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[r][lane]);
-                    s = fma2(exp2_2(mul2(v.x, rate[k])), s, mul2(v.y, *reinterpret_cast<const f2*>(&sm.bc[r][n])));
+                for (int r = 0; r < BWD_ROWS; r++) {
+                    const int row = (sub - 1) * BWD_ROWS + r;
+                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[row][lane]);
+#pragma unroll
+                    for (int k = 0; k < K; k++)
+                        s[k] = fma2(exp2_2(mul2(v.x, rate[k])), s[k], mul2(v.y, *reinterpret_cast<const f2*>(&sm.bc[row][warp * K + k])));
                 }
-                *reinterpret_cast<f2*>(&sm.h[n][lane]) = s;
+#pragma unroll
+                for (int k = 0; k < K; k++) *reinterpret_cast<f2*>(&sm.h[sub - 1][warp * K + k][lane]) = s[k];
             }
         }
 #pragma unroll 1
         for (int sub = subs - 1; sub >= 0; sub--) {
-            const int q = sub * SSM_ROWS;
-            const float2* front = sub ? &sm.h[0][lane] : &sm.h0[buf][0][lane];
-            f2 dl[SSM_ROWS], dx[SSM_ROWS], e[SSM_ROWS], sb[SSM_ROWS], su[SSM_ROWS];
-            [[maybe_unused]] f2 y[SSM_ROWS];
+            const int q = sub * BWD_ROWS, turn = sub & 1;
+            const float2* front = sub ? &sm.h[sub - 1][0][lane] : &sm.h0[buf][0][lane];
+            f2 dl[BWD_ROWS], dx[BWD_ROWS], e[BWD_ROWS], sb[BWD_ROWS], su[BWD_ROWS];
+            [[maybe_unused]] f2 y[BWD_ROWS];
 #pragma unroll
-            for (int r = 0; r < SSM_ROWS; r++) {
+            for (int r = 0; r < BWD_ROWS; r++) {
                 const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[q + r][lane]);
                 dl[r] = v.x;
                 dx[r] = v.y;
@@ -281,23 +302,22 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
-                if (n >= p.N) break;
-                f2 a[SSM_ROWS], u[SSM_ROWS], s = *reinterpret_cast<const f2*>(front + n * 32);
-                float part[SSM_ROWS];
+                if (!FULL && n >= p.N) break;           // (FULL: N = K W.  A branch here would keep the states' chains apart)
+                f2 a[BWD_ROWS], u[BWD_ROWS], s = *reinterpret_cast<const f2*>(front + n * 32);
+                float pc[BWD_ROWS], pb[BWD_ROWS];
 #pragma unroll
-                for (int r = 0; r < SSM_ROWS; r++) {
+                for (int r = 0; r < BWD_ROWS; r++) {
                     const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&sm.bc[q + r][n]);
                     a[r] = exp2_2(mul2(dl[r], rate[k]));
                     u[r] = mul2(a[r], s);
                     s = fma2(dx[r], bc.x, u[r]);
                     if (GATED) y[r] = fma2(s, bc.y, y[r]);
                     const float2 c = unpack2(mul2(e[r], s));
-                    part[r] = c.x + c.y;
+                    pc[r] = c.x + c.y;
                 }
-                const float dc = butterfly8(part, lane);
                 f2 g = G[k];
 #pragma unroll
-                for (int r = SSM_ROWS - 1; r >= 0; r--) {
+                for (int r = BWD_ROWS - 1; r >= 0; r--) {
                     const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&sm.bc[q + r][n]);
                     g = fma2(bc.y, e[r], g);
                     sb[r] = fma2(g, bc.x, sb[r]);
@@ -305,30 +325,30 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
                     su[r] = fma2(w, rate[k], su[r]);
                     dA[k] = fma2(dl[r], w, dA[k]);
                     const float2 c = unpack2(mul2(g, dx[r]));
-                    part[r] = c.x + c.y;
+                    pb[r] = c.x + c.y;
                     g = mul2(a[r], g);
                 }
                 G[k] = g;
-                const float db = butterfly8(part, lane);
-                if ((lane & 3) == 0) sm.bcg[sub][lane >> 2][n] = make_float2(db, dc);
+                const float2 sums = butterfly<BWD_ROWS>(pb, pc, lane);
+                if (lane % (32 / BWD_ROWS) == 0) sm.bcg[turn][lane / (32 / BWD_ROWS)][n] = sums;
             }
 #pragma unroll
-            for (int r = 0; r < SSM_ROWS; r++) {
-                *reinterpret_cast<f2*>(&sm.red[sub][0][warp][r][lane]) = sb[r];
-                *reinterpret_cast<f2*>(&sm.red[sub][1][warp][r][lane]) = su[r];
-                if (GATED) *reinterpret_cast<f2*>(&sm.red[sub][2][warp][r][lane]) = y[r];
+            for (int r = 0; r < BWD_ROWS; r++) {
+                *reinterpret_cast<f2*>(&sm.red[turn][0][warp][r][lane]) = sb[r];
+                *reinterpret_cast<f2*>(&sm.red[turn][1][warp][r][lane]) = su[r];
+                if (GATED) *reinterpret_cast<f2*>(&sm.red[turn][2][warp][r][lane]) = y[r];
             }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < SIT; i++) {
                 const int r = warp + W * i, t = tc + q + r;
-                if (t < t_end) {
+                if (t < t_end && (SIT * W == BWD_ROWS || r < BWD_ROWS)) {
                     f2 vs = 0, vu = 0, vy = 0;
 #pragma unroll
                     for (int w = 0; w < W; w++) {
-                        vs = add2(vs, *reinterpret_cast<const f2*>(&sm.red[sub][0][w][r][lane]));
-                        vu = add2(vu, *reinterpret_cast<const f2*>(&sm.red[sub][1][w][r][lane]));
-                        if (GATED) vy = add2(vy, *reinterpret_cast<const f2*>(&sm.red[sub][2][w][r][lane]));
+                        vs = add2(vs, *reinterpret_cast<const f2*>(&sm.red[turn][0][w][r][lane]));
+                        vu = add2(vu, *reinterpret_cast<const f2*>(&sm.red[turn][1][w][r][lane]));
+                        if (GATED) vy = add2(vy, *reinterpret_cast<const f2*>(&sm.red[turn][2][w][r][lane]));
                     }
                     const float2 xv = to_float2<T>(sm.raw[buf][0][q + r][lane]);
                     const f2 x = pack2(xv.x, xv.y), ev = *reinterpret_cast<const f2*>(&sm.e[q + r][lane]);
@@ -353,10 +373,10 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
                 }
             }
 #pragma unroll
-            for (int i = 0; i < (SSM_ROWS * NP + 32 * W - 1) / (32 * W); i++) {
+            for (int i = 0; i < (BWD_ROWS * NP + 32 * W - 1) / (32 * W); i++) {
                 const int r = bt + BSTEP * i, t = tc + q + r;
-                if (r < SSM_ROWS && t < t_end && bn < p.N)
-                    p.bc_part[((static_cast<size_t>(blockIdx.x) * p.nb + bl) * p.S + t) * p.N + bn] = sm.bcg[sub][r][bn];
+                if (r < BWD_ROWS && t < t_end && bn < p.N)
+                    p.bc_part[((static_cast<size_t>(blockIdx.x) * p.nb + bl) * p.S + t) * p.N + bn] = sm.bcg[turn][r][bn];
             }
         }
     }
@@ -451,8 +471,9 @@ template <typename T, int K, int W>
 cudaError_t launch_ssm_bwd(SsmBwdArgs a, const SsmBwdWs& w, void* dB, void* dC, cudaStream_t st) {
     const unsigned tiles = static_cast<unsigned>(a.G * a.tiles_g);
     constexpr size_t smem = sizeof(SsmBwdSmem<T, K, W>);
-    auto kern = a.z ? (a.pairs ? ssm_bwd_kernel<T, K, W, true, true> : ssm_bwd_kernel<T, K, W, true, false>)
-                     : (a.pairs ? ssm_bwd_kernel<T, K, W, false, true> : ssm_bwd_kernel<T, K, W, false, false>);
+    const bool full = a.pairs && a.N == K * W;
+    auto kern = a.z ? (full ? ssm_bwd_kernel<T, K, W, true, true, true> : a.pairs ? ssm_bwd_kernel<T, K, W, true, true, false> : ssm_bwd_kernel<T, K, W, true, false, false>)
+                    : (full ? ssm_bwd_kernel<T, K, W, false, true, true> : a.pairs ? ssm_bwd_kernel<T, K, W, false, true, false> : ssm_bwd_kernel<T, K, W, false, false, false>);
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     for (int b0 = 0; b0 < a.Bt && ce == cudaSuccess; b0 += w.nb) {
         a.b0 = b0;
