@@ -183,7 +183,7 @@ def require_cuda(*tensors):
 def require_one_cuda_device(first, *others):
     """The CUDA device that all of the tensors (None: left out) live on."""
     dev = first.device
-    if dev.type != "cuda":
+    if not first.is_cuda:
         raise RuntimeError("these kernels need CUDA tensors; there is no CPU path")
     for t in others:
         if t is not None and t.device != dev:
@@ -199,6 +199,10 @@ def device_guard(dev):
     return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def scratch(nbytes: int, dev):
     """(tensor, address, bytes) of scratch memory of one call's own.  Unlike ``workspace`` nothing is kept between calls, so a
     captured graph owns its scratch and no later call can free or reuse it."""
@@ -208,7 +212,13 @@ def scratch(nbytes: int, dev):
     return buf, buf.data_ptr(), nbytes
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (absent in builds without CUDA)
+
+
 def stream_ptr(dev) -> int:
+    """Address of the device's current stream; asked for directly, without a Stream object, where torch offers that."""
+    if _raw_stream is not None and dev.index is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 

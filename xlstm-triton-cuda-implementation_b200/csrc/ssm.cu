@@ -1,6 +1,7 @@
 // Selective state space scan: forward over prompts, and the step for a few new tokens (ssm_common.cuh has the formulas and the
 // layout of the work).
 #include "ssm_common.cuh"
+#include "vec_cvt.cuh"
 
 namespace mlstm {
 namespace {
@@ -268,79 +269,160 @@ cudaError_t launch_ssm_fwd_n(const SsmFwdArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------------- a few new tokens
 constexpr int STEP_TOKENS = 8;
 constexpr int STEP_THREADS = 128;
+constexpr int STEP_CH = 4;           // channels per group of lanes
 
 struct SsmStepArgs : SsmArgs {
     const float* initial;
     void* y;
     float* state_out;
-    int lanes;                       // lanes per channel (a power of two), four states each
-    int vec;                         // states can be accessed four at a time
 };
 
-template <typename T>
+// L lanes share STEP_CH neighbouring channels, four states of each per lane; every channel's input, step and output are one lane's
+// (lane i % L for channel i), which hands them to the others.  A group works on several sequences, one after the other, so
+// that A is read once for them.  VEC: N = 4 L, states and B, C in whole pieces, all four channels in one group.
+// Bound by the states, read and written once: 256 sequences x 4096 channels x 16 states, 134 MB.
+template <typename T, int L, bool VEC>
 __global__ void __launch_bounds__(STEP_THREADS) ssm_step_kernel(const SsmStepArgs p) {
+    constexpr int CH = STEP_CH, OWN = (CH + L - 1) / L;      // channels whose values this lane takes
     grid_dep_wait();
     grid_dep_launch();
-    const int L = p.lanes, per = STEP_THREADS / L, b = blockIdx.y;
-    const int sub = threadIdx.x & (L - 1), c = blockIdx.x * per + static_cast<int>(threadIdx.x) / L, n0 = sub * 4;
-    const bool on = c < p.Ch;
-    const int cc = on ? c : 0, nn = on ? max(0, min(4, p.N - n0)) : 0, g = cc / p.P;
-    float h[4] = {0.f, 0.f, 0.f, 0.f}, rate[4] = {0.f, 0.f, 0.f, 0.f};
-    const size_t at = static_cast<size_t>(cc) * p.N + n0, hb = static_cast<size_t>(b) * p.Ch * p.N + at;
-    if (p.vec && nn == 4) {
-        const float4 r = *reinterpret_cast<const float4*>(p.A + at);
-        rate[0] = r.x; rate[1] = r.y; rate[2] = r.z; rate[3] = r.w;
-        if (p.initial) {
-            const float4 v = *reinterpret_cast<const float4*>(p.initial + hb);
-            h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
-        }
-    } else {
+    const int lane = threadIdx.x & 31, sub = lane & (L - 1), lead = lane - sub;
+    const int c0 = ((blockIdx.x * STEP_THREADS + threadIdx.x) / L) * CH, n0 = sub * 4;
+    const int nn = max(0, min(4, p.N - n0));
+    int c[CH];
+    bool on[CH];
+    float rate[CH][4], bias[OWN], skip[OWN];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j < nn) {
-                rate[j] = p.A[at + j];
-                if (p.initial) h[j] = p.initial[hb + j];
-            }
+    for (int i = 0; i < CH; i++) {
+        on[i] = c0 + i < p.Ch;
+        c[i] = on[i] ? c0 + i : 0;
+        const float* A = p.A + static_cast<size_t>(c[i]) * p.N + n0;
+        if (VEC) {
+            const float4 r = on[i] ? *reinterpret_cast<const float4*>(A) : make_float4(0.f, 0.f, 0.f, 0.f);
+            rate[i][0] = r.x; rate[i][1] = r.y; rate[i][2] = r.z; rate[i][3] = r.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) rate[i][j] = j < nn ? A[j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) rate[i][j] = decay_rate(rate[i][j]);
     }
+    int mine[OWN];                           // (0 where there is none: read, and not written)
+    bool have[OWN];
 #pragma unroll
-    for (int j = 0; j < 4; j++) rate[j] = decay_rate(rate[j]);
-    const float bias = p.bias ? p.bias[cc] : 0.f, skip = p.D ? p.D[cc] : 0.f;
-    for (int t = 0; t < p.S; t++) {
-        const float x = to_f32<T>(static_cast<const T*>(p.x)[b * p.sx.b + t * p.sx.t + cc]);
-        float d = to_f32<T>(static_cast<const T*>(p.dt)[b * p.sdt.b + t * p.sdt.t + cc]) + bias;
-        if (p.softplus) d = softplus_f(d);
-        const float dx = d * x;
-        const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + t * p.sB.t + static_cast<long long>(g) * p.N + n0;
-        const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + t * p.sC.t + static_cast<long long>(g) * p.N + n0;
-        float y = 0.f;
+    for (int o = 0; o < OWN; o++) {
+        const int i = o * L + sub;
+        have[o] = i < CH && c0 + i < p.Ch;
+        mine[o] = have[o] ? c0 + i : 0;
+        bias[o] = p.bias ? p.bias[mine[o]] : 0.f;
+        skip[o] = p.D ? p.D[mine[o]] : 0.f;
+    }
+    for (int b = blockIdx.y; b < p.Bt; b += gridDim.y) {
+        float h[CH][4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j < nn) {
-                h[j] = fmaf(fast_exp2(d * rate[j]), h[j], dx * to_f32<T>(Bp[j]));
-                y = fmaf(h[j], to_f32<T>(Cp[j]), y);
+        for (int i = 0; i < CH; i++) {
+            const float* H = p.initial + (static_cast<size_t>(b) * p.Ch + c[i]) * p.N + n0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[i][j] = 0.f;
+            if (p.initial && on[i]) {
+                if (VEC) {
+                    const float4 v = *reinterpret_cast<const float4*>(H);
+                    h[i][0] = v.x; h[i][1] = v.y; h[i][2] = v.z; h[i][3] = v.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (j < nn) h[i][j] = H[j];
+                }
             }
         }
-        for (int o = L >> 1; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-        if (on && sub == 0) {
-            if (p.D) y = fmaf(skip, x, y);
-            if (p.z) y *= silu_f(to_f32<T>(static_cast<const T*>(p.z)[b * p.sz.b + t * p.sz.t + cc]));
-            static_cast<T*>(p.y)[(static_cast<size_t>(b) * p.S + t) * p.Ch + c] = from_f32<T>(y);
-        }
-    }
-    if (p.state_out) {
-        if (p.vec && nn == 4) *reinterpret_cast<float4*>(p.state_out + hb) = make_float4(h[0], h[1], h[2], h[3]);
-        else {
+        for (int t = 0; t < p.S; t++) {
+            float x[OWN], d[OWN], gate[OWN];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < nn) p.state_out[hb + j] = h[j];
+            for (int o = 0; o < OWN; o++) {
+                x[o] = to_f32<T>(static_cast<const T*>(p.x)[b * p.sx.b + t * p.sx.t + mine[o]]);
+                d[o] = to_f32<T>(static_cast<const T*>(p.dt)[b * p.sdt.b + t * p.sdt.t + mine[o]]) + bias[o];
+                if (p.z) gate[o] = to_f32<T>(static_cast<const T*>(p.z)[b * p.sz.b + t * p.sz.t + mine[o]]);
+            }
+            float Bv[4], Cv[4];
+            const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + t * p.sB.t + n0;
+            const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + t * p.sC.t + n0;
+            auto vectors = [&](int g) {
+                const T *B = Bp + static_cast<long long>(g) * p.N, *C = Cp + static_cast<long long>(g) * p.N;
+                if (VEC) {
+                    to_floats<T, 4>(load_vec<T, 4>(B), Bv);
+                    to_floats<T, 4>(load_vec<T, 4>(C), Cv);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        Bv[j] = j < nn ? to_f32<T>(B[j]) : 0.f;
+                        Cv[j] = j < nn ? to_f32<T>(C[j]) : 0.f;
+                    }
+                }
+            };
+            if (VEC) vectors(c[0] / p.P);
+#pragma unroll
+            for (int o = 0; o < OWN; o++)
+                if (p.softplus) d[o] = softplus_f(d[o]);
+            float y[OWN];
+#pragma unroll
+            for (int o = 0; o < OWN; o++) y[o] = 0.f;
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const float di = __shfl_sync(0xffffffffu, d[i / L], lead + i % L), xi = __shfl_sync(0xffffffffu, x[i / L], lead + i % L);
+                if (!VEC) vectors(c[i] / p.P);
+                const float dx = di * xi;
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (VEC || j < nn) {
+                        h[i][j] = fmaf(fast_exp2(di * rate[i][j]), h[i][j], dx * Bv[j]);
+                        s = fmaf(h[i][j], Cv[j], s);
+                    }
+                }
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (i % L == sub) y[i / L] = s;
+            }
+#pragma unroll
+            for (int o = 0; o < OWN; o++) {
+                if (p.D) y[o] = fmaf(skip[o], x[o], y[o]);
+                if (p.z) y[o] *= gate[o] * sigmoid_f(gate[o]);
+                if (have[o]) static_cast<T*>(p.y)[(static_cast<size_t>(b) * p.S + t) * p.Ch + mine[o]] = from_f32<T>(y[o]);
+            }
+        }
+        if (p.state_out) {
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                float* H = p.state_out + (static_cast<size_t>(b) * p.Ch + c[i]) * p.N + n0;
+                if (!on[i]) continue;
+                if (VEC) *reinterpret_cast<float4*>(H) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
+                else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (j < nn) H[j] = h[i][j];
+                }
+            }
         }
     }
 }
 
+template <typename T, int L>
+cudaError_t launch_ssm_step_l(const SsmStepArgs& a, bool vec, cudaStream_t st) {
+    const int per = STEP_THREADS / L * STEP_CH, gx = ceil_div(a.Ch, per);
+    // as many sequences per group as leave every SM some sixteen blocks
+    int gy = ceil_div(148 * 16, gx);
+    gy = gy < a.Bt ? gy : a.Bt;
+    gy = ceil_div(a.Bt, ceil_div(a.Bt, gy));
+    return vec && a.N == 4 * L ? launch_plain(ssm_step_kernel<T, L, true>, dim3(gx, gy), dim3(STEP_THREADS), 0, st, a)
+                               : launch_plain(ssm_step_kernel<T, L, false>, dim3(gx, gy), dim3(STEP_THREADS), 0, st, a);
+}
 template <typename T>
-cudaError_t launch_ssm_step(const SsmStepArgs& a, cudaStream_t st) {
-    const int per = STEP_THREADS / a.lanes;
-    return launch_plain(ssm_step_kernel<T>, dim3(ceil_div(a.Ch, per), a.Bt), dim3(STEP_THREADS), 0, st, a);
+cudaError_t launch_ssm_step(const SsmStepArgs& a, bool vec, cudaStream_t st) {
+    if (a.N <= 4) return launch_ssm_step_l<T, 1>(a, vec, st);
+    if (a.N <= 8) return launch_ssm_step_l<T, 2>(a, vec, st);
+    if (a.N <= 16) return launch_ssm_step_l<T, 4>(a, vec, st);
+    if (a.N <= 32) return launch_ssm_step_l<T, 8>(a, vec, st);
+    return launch_ssm_step_l<T, 16>(a, vec, st);
 }
 
 // How many segments the positions are cut into: one where the channels alone fill the chip.  Cutting costs a second pass over
@@ -465,11 +547,12 @@ int mlstm_ssm_fwd(const void* x, const void* dt, const float* A, const void* Bv,
         SsmStepArgs a;
         static_cast<SsmArgs&>(a) = base;
         a.initial = initial; a.y = y; a.state_out = state_out;
-        a.lanes = 1;
-        while (a.lanes * 4 < N) a.lanes *= 2;
-        a.vec = N % 4 == 0 && ssm_aligned(A, 16) && ssm_aligned(initial, 16) && ssm_aligned(state_out, 16);
-        ce = dtype == MLSTM_DT_F32 ? launch_ssm_step<float>(a, st)
-             : dtype == MLSTM_DT_F16 ? launch_ssm_step<__half>(a, st) : launch_ssm_step<__nv_bfloat16>(a, st);
+        // whole pieces of four states, and of four values of B and C; four channels of one group
+        const long long strides4 = a.sB.b | a.sB.t | a.sC.b | a.sC.t;
+        const bool vec = N % 4 == 0 && a.P % STEP_CH == 0 && (strides4 & 3) == 0 && ssm_aligned(A, 16) && ssm_aligned(initial, 16) &&
+                         ssm_aligned(state_out, 16) && ssm_aligned(Bv, 4 * es) && ssm_aligned(Cv, 4 * es);
+        ce = dtype == MLSTM_DT_F32 ? launch_ssm_step<float>(a, vec, st)
+             : dtype == MLSTM_DT_F16 ? launch_ssm_step<__half>(a, vec, st) : launch_ssm_step<__nv_bfloat16>(a, vec, st);
     } else {
         SsmFwdArgs a;
         static_cast<SsmArgs&>(a) = base;

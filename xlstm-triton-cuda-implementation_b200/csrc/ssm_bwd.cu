@@ -26,10 +26,7 @@ struct SsmBwdArgs : SsmArgs {
     int b0, nb;                     // batches of this launch: b0 .. b0 + nb - 1
 };
 
-#ifndef BR
-#define BR 8
-#endif
-constexpr int BWD_ROWS = BR;                            // positions whose states are held in registers at a time
+constexpr int BWD_ROWS = 8;                            // positions whose states are held in registers at a time
 constexpr int BWD_SUBS = SSM_CK / BWD_ROWS;
 
 template <typename T, int K, int W>
@@ -435,7 +432,11 @@ struct SsmParamOut {
 };
 
 constexpr size_t SSM_BWD_PART_MAX = 512u << 20;     // bytes of dB, dC partials in scratch at one time (at least one batch entry)
-constexpr int SSM_BWD_CTAS = 2;                     // CTAs that an SM is filled with
+// Four states per warp and four warps: two CTAs fill an SM's registers.  Where the channels give at most one CTA to an SM, or there are
+// more states, eight warps (with two states each, 4 x 4096 x 4096: 2.69 against 2.33 ms for forward and backward, but
+// 2 x 2048 x 4096: 0.74 against 0.83 ms).
+bool ssm_bwd_wide(const SsmArgs& a) { return a.N > 16 || (a.N > 8 && static_cast<long long>(a.G) * a.tiles_g * a.Bt <= 148); }
+void ssm_bwd_cut(SsmArgs& a) { ssm_cut(a, ssm_bwd_wide(a) ? 1 : 2); }
 
 struct SsmBwdWs {
     float *seg_end, *seg_sum, *param;
@@ -491,7 +492,7 @@ template <typename T>
 cudaError_t launch_ssm_bwd_n(const SsmBwdArgs& a, const SsmBwdWs& w, void* dB, void* dC, cudaStream_t st) {
     if (a.N <= 4) return launch_ssm_bwd<T, 1, 4>(a, w, dB, dC, st);
     if (a.N <= 8) return launch_ssm_bwd<T, 2, 4>(a, w, dB, dC, st);
-    if (a.N <= 16) return launch_ssm_bwd<T, 4, 4>(a, w, dB, dC, st);
+    if (a.N <= 16) return ssm_bwd_wide(a) ? launch_ssm_bwd<T, 2, 8>(a, w, dB, dC, st) : launch_ssm_bwd<T, 4, 4>(a, w, dB, dC, st);
     if (a.N <= 32) return launch_ssm_bwd<T, 4, 8>(a, w, dB, dC, st);
     return launch_ssm_bwd<T, 8, 8>(a, w, dB, dC, st);
 }
@@ -509,7 +510,7 @@ size_t mlstm_ssm_bwd_workspace(int B, int S, int C, int G, int N) {
     if (ssm_fill(a, any, any, static_cast<const float*>(any), any, any, nullptr, nullptr, nullptr, nullptr, B, S, C, G, N,
                  MLSTM_DT_F32, 0) != MLSTM_OK)
         return 0;
-    ssm_cut(a, SSM_BWD_CTAS);
+    ssm_bwd_cut(a);
     return ssm_bwd_carve(nullptr, a).bytes;
 }
 
@@ -529,7 +530,7 @@ int mlstm_ssm_bwd(const void* dy, const void* x, const void* dt, const float* A,
     for (const float* q : {A, D, dt_bias, static_cast<const float*>(dA), static_cast<const float*>(dD), static_cast<const float*>(d_dt_bias)})
         if (!ssm_aligned(q, 4)) return MLSTM_E_ALIGN;
     if (!ssm_aligned(checkpoints, 8)) return MLSTM_E_ALIGN;
-    ssm_cut(a, SSM_BWD_CTAS);
+    ssm_bwd_cut(a);
     const SsmBwdWs w = ssm_bwd_carve(workspace, a);
     if (!workspace || workspace_bytes < w.bytes || !ssm_aligned(workspace, 16)) return MLSTM_E_WORKSPACE;
     a.seg_end = w.seg_end; a.seg_sum = w.seg_sum; a.param_part = w.param; a.bc_part = w.bc;

@@ -22,10 +22,6 @@ from . import _lib
 __all__ = ["residual_rms_norm", "residual_rms_norm_backward", "residual_rms_norm_quantized"]
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
 def _check(x, weight, residual):
     """(device, rows, D, groups, inner) of x with this weight."""
     if x.dim() < 1 or x.numel() == 0:
@@ -58,7 +54,7 @@ def _forward(x, weight, residual, eps, out, scale, block):
     total = None if residual is None else torch.empty_like(residual)
     stream = x if residual is None else residual
     with _lib.device_guard(dev):
-        rc = _lib.lib().mlstm_rms_fwd(x.data_ptr(), _ptr(residual), _ptr(weight), out.data_ptr(), _ptr(total), _ptr(scale), rows, D,
+        rc = _lib.lib().mlstm_rms_fwd(x.data_ptr(), _lib.ptr(residual), _lib.ptr(weight), out.data_ptr(), _lib.ptr(total), _lib.ptr(scale), rows, D,
                                       groups, inner, block, eps, _lib.dtype_code(x), _lib.dtype_code(stream),
                                       0 if weight is None else _lib.dtype_code(weight), 0 if scale is not None else _lib.dtype_code(out),
                                       _lib.stream_ptr(dev))
@@ -89,8 +85,8 @@ def residual_rms_norm_backward(dy, s, weight=None, ds=None, eps=1e-6, x_dtype=No
     L = _lib.lib()
     ws, at, nbytes = _lib.scratch(0 if weight is None else L.mlstm_rms_bwd_workspace(rows, D, groups, inner), dev)
     with _lib.device_guard(dev):
-        rc = L.mlstm_rms_bwd(dy.data_ptr(), _ptr(ds), s.data_ptr(), _ptr(weight), dx.data_ptr(), None if dres is dx else dres.data_ptr(),
-                             _ptr(dweight), at, nbytes, rows, D, groups, inner, eps, _lib.dtype_code(dx), _lib.dtype_code(s),
+        rc = L.mlstm_rms_bwd(dy.data_ptr(), _lib.ptr(ds), s.data_ptr(), _lib.ptr(weight), dx.data_ptr(), None if dres is dx else dres.data_ptr(),
+                             _lib.ptr(dweight), at, nbytes, rows, D, groups, inner, eps, _lib.dtype_code(dx), _lib.dtype_code(s),
                              0 if weight is None else _lib.dtype_code(weight), _lib.dtype_code(dy), _lib.stream_ptr(dev))
     _lib.check(rc, "mlstm_rms_bwd")
     return dx, dres, dweight
@@ -99,7 +95,7 @@ def residual_rms_norm_backward(dy, s, weight=None, ds=None, eps=1e-6, x_dtype=No
 class _ResidualRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, out_dtype):
-        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
         total = _forward(x, weight, residual, eps, y, None, 0)
         ctx.save_for_backward(x if total is None else total, weight)
         ctx.eps, ctx.x_dtype, ctx.with_residual = eps, x.dtype, residual is not None
@@ -122,9 +118,9 @@ def residual_rms_norm(x, weight=None, residual=None, eps=1e-6, out_dtype=None):
     stream = x if residual is None else residual
     if out_dtype not in (torch.float32, torch.float16, torch.bfloat16) or (out_dtype != stream.dtype and stream.dtype != torch.float32):
         raise TypeError("out_dtype must be the type of the stream (x, or the residual), or any where that is float32")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in (x, weight, residual) if t is not None]):
         return _ResidualRmsNorm.apply(x, weight, residual, float(eps), out_dtype)
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    y = torch.empty_like(x) if out_dtype is x.dtype and x.is_contiguous() else x.new_empty(x.shape, dtype=out_dtype)
     total = _forward(x, weight, residual, float(eps), y, None, 0)
     return y if total is None else (y, total)
 
@@ -133,7 +129,7 @@ def residual_rms_norm_quantized(x, weight=None, residual=None, eps=1e-6, block=N
     """(q, scale), with a residual (q, scale, s).  q: float8_e4m3fn, x's shape; scale: float32, x's shape with the last dimension
     D / block: the largest magnitude of a row, or of each ``block`` (32, 64, 128) of its values, divided by 448 (1 where all are
     zero).  Values round to the nearest; a block with an infinity or a NaN gets that as its scale."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in (x, weight, residual) if t is not None]):
         raise ValueError("the quantized norm has no gradients")
     D = x.shape[-1] if x.dim() else 0
     if block is not None and (block not in (32, 64, 128) or D % block):

@@ -24,33 +24,35 @@ __all__ = ["short_convolution", "short_convolution_backward"]
 _ACTIVATIONS = {None: 0, "silu": 1}
 
 
-def _strides(t, name):
-    """Element strides (batch, position) of a [B, S, C] tensor whose last dimension is contiguous."""
-    s = t.stride()
-    if s[2] != 1 and t.shape[2] != 1:
-        raise RuntimeError(f"the last dimension of {name} must be contiguous")
-    return s[0], s[1]
+_Strides = ctypes.c_longlong * 2
 
 
 def _check(x, weight, bias, activation):
-    if x.dim() != 3 or 0 in x.shape:
+    """(device, strides of x or None where it is contiguous)"""
+    if x.dim() != 3 or not x.numel():
         raise ValueError("x must have the shape [B, S, C] with at least one of each")
-    if weight.dim() != 2 or weight.shape[0] != x.shape[2] or not 2 <= weight.shape[1] <= 4:
+    C = x.shape[2]
+    if weight.dim() != 2 or weight.shape[0] != C or not 2 <= weight.shape[1] <= 4:
         raise ValueError("weight must have the shape [C, W] with W = 2, 3 or 4")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError("bias must have the shape [C]")
-    if weight.dtype not in (x.dtype, torch.float32) or (bias is not None and bias.dtype != weight.dtype):
-        raise TypeError("weight and bias must share one element type: x's or float32")
     if activation not in _ACTIVATIONS:
         raise ValueError('activation must be None or "silu"')
+    wdt = weight.dtype
+    if wdt is not x.dtype and wdt is not torch.float32:
+        raise TypeError("weight and bias must share one element type: x's or float32")
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != C:
+            raise ValueError("bias must have the shape [C]")
+        if bias.dtype is not wdt:
+            raise TypeError("weight and bias must share one element type: x's or float32")
     dev = _lib.require_one_cuda_device(x, weight, bias)
     if not weight.is_contiguous() or (bias is not None and not bias.is_contiguous()):
         raise RuntimeError("weight and bias must be contiguous")
-    return dev, (ctypes.c_longlong * 2)(*_strides(x, "x"))
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+    if x.is_contiguous():
+        return dev, None
+    s = x.stride()
+    if s[2] != 1 and C != 1:
+        raise RuntimeError("the last dimension of x must be contiguous")
+    return dev, _Strides(s[0], s[1])
 
 
 def _forward(x, weight, bias, activation, initial, state_out):
@@ -60,10 +62,10 @@ def _forward(x, weight, bias, activation, initial, state_out):
     for name, t in (("initial", initial), ("state_out", state_out)):
         if t is not None and (t.shape != (B, W - 1, C) or t.dtype != x.dtype or not t.is_contiguous() or t.device != dev):
             raise ValueError(f"{name} must be a contiguous [B, W - 1, C] tensor of x's type and device")
-    y = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    y = torch.empty_like(x) if strides is None else x.new_empty((B, S, C))
     with _lib.device_guard(dev):
-        rc = _lib.lib().mlstm_conv_fwd(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(initial), strides, y.data_ptr(),
-                                       _ptr(state_out), B, S, C, W, _lib.dtype_code(x), _lib.dtype_code(weight),
+        rc = _lib.lib().mlstm_conv_fwd(x.data_ptr(), weight.data_ptr(), _lib.ptr(bias), _lib.ptr(initial), strides, y.data_ptr(),
+                                       _lib.ptr(state_out), B, S, C, W, _lib.dtype_code(x), _lib.dtype_code(weight),
                                        _ACTIVATIONS[activation], _lib.stream_ptr(dev))
     _lib.check(rc, "mlstm_conv_fwd")
     return y
@@ -79,13 +81,13 @@ def short_convolution_backward(dy, x, weight, bias=None, activation=None):
     W = weight.shape[1]
     dt = _lib.dtype_code(x)
     L = _lib.lib()
-    dx = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    dx = torch.empty_like(x) if strides is None else x.new_empty((B, S, C))
     dweight = torch.empty_like(weight)
     dbias = None if bias is None else torch.empty_like(bias)
     ws, at, nbytes = _lib.scratch(L.mlstm_conv_bwd_workspace(B, S, C, W, dt), dev)
     with _lib.device_guard(dev):
-        rc = L.mlstm_conv_bwd(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(bias), strides, dx.data_ptr(),
-                              dweight.data_ptr(), _ptr(dbias), at, nbytes, B, S, C, W, dt, _lib.dtype_code(weight),
+        rc = L.mlstm_conv_bwd(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _lib.ptr(bias), strides, dx.data_ptr(),
+                              dweight.data_ptr(), _lib.ptr(dbias), at, nbytes, B, S, C, W, dt, _lib.dtype_code(weight),
                               _ACTIVATIONS[activation], _lib.stream_ptr(dev))
     _lib.check(rc, "mlstm_conv_bwd")
     return dx, dweight, dbias
@@ -118,5 +120,6 @@ def short_convolution(x, weight, bias=None, activation=None, initial=None, retur
     if state_out is None:
         if x.dim() != 3 or weight.dim() != 2:
             raise ValueError("x must have the shape [B, S, C] and weight [C, W]")
-        state_out = torch.empty((x.shape[0], max(weight.shape[1] - 1, 0), x.shape[2]), dtype=x.dtype, device=x.device)
+        state_out = (torch.empty_like(initial) if initial is not None and initial.is_contiguous()
+                     else x.new_empty((x.shape[0], max(weight.shape[1] - 1, 0), x.shape[2])))
     return _forward(x, weight, bias, activation, initial, state_out), state_out
