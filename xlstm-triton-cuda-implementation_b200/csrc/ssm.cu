@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArg
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
-                if (n < p.N) h[k] = fma2(exp2_2(mul2(sum, rate[k])), h[k], *reinterpret_cast<const f2*>(seg_state(j, n)));
+                if (n < p.N) h[k] = fma2(decay2(sum, rate[k]), h[k], *reinterpret_cast<const f2*>(seg_state(j, n)));
             }
         }
     }
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArg
 #pragma unroll
                 for (int r = 0; r < SSM_ROWS; r++) {
                     const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&sm.bc[buf][half + r][warp * K + k]);
-                    s = fma2(exp2_2(mul2(dl[r], rate[k])), s, mul2(dx[r], bc.x));
+                    s = fma2(decay2(dl[r], rate[k]), s, mul2(dx[r], bc.x));
                     if (OUT) y[r] = fma2(s, bc.y, y[r]);
                 }
                 h[k] = s;
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(STEP_THREADS) ssm_step_kernel(const SsmStepArg
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if (VEC || j < nn) {
-                        h[i][j] = fmaf(fast_exp2(di * rate[i][j]), h[i][j], dx * Bv[j]);
+                        h[i][j] = fmaf(decay_f(di, rate[i][j]), h[i][j], dx * Bv[j]);
                         s = fmaf(h[i][j], Cv[j], s);
                     }
                 }

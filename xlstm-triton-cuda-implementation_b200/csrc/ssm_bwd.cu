@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
 #pragma unroll
             for (int r = TILE - 1; r >= 0; r--) {
                 const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm_d[r][lane]);
-                G[k] = mul2(exp2_2(mul2(v.x, rate[k])), fma2(v.y, *reinterpret_cast<const f2*>(&sm_c[r][warp * K + k]), G[k]));
+                G[k] = mul2(decay2(v.x, rate[k]), fma2(v.y, *reinterpret_cast<const f2*>(&sm_c[r][warp * K + k]), G[k]));
             }
         }
         if (warp == 0) {
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
         for (int k = 0; k < K; k++) {
             const int n = warp * K + k;
             if (n < p.N)
-                G[k] = fma2(exp2_2(mul2(sum, rate[k])), G[k], *reinterpret_cast<const f2*>(p.seg_end + (sj * p.N + n) * p.Cpad + ch.cp));
+                G[k] = fma2(decay2(sum, rate[k]), G[k], *reinterpret_cast<const f2*>(p.seg_end + (sj * p.N + n) * p.Cpad + ch.cp));
         }
     }
 
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
                     const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.dl[row][lane]);
 #pragma unroll
                     for (int k = 0; k < K; k++)
-                        s[k] = fma2(exp2_2(mul2(v.x, rate[k])), s[k], mul2(v.y, *reinterpret_cast<const f2*>(&sm.bc[row][warp * K + k])));
+                        s[k] = fma2(decay2(v.x, rate[k]), s[k], mul2(v.y, *reinterpret_cast<const f2*>(&sm.bc[row][warp * K + k])));
                 }
 #pragma unroll
                 for (int k = 0; k < K; k++) *reinterpret_cast<f2*>(&sm.h[sub - 1][warp * K + k][lane]) = s[k];
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
 #pragma unroll
                 for (int r = 0; r < BWD_ROWS; r++) {
                     const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&sm.bc[q + r][n]);
-                    a[r] = exp2_2(mul2(dl[r], rate[k]));
+                    a[r] = decay2(dl[r], rate[k]);
                     u[r] = mul2(a[r], s);
                     s = fma2(dx[r], bc.x, u[r]);
                     if (GATED) y[r] = fma2(s, bc.y, y[r]);

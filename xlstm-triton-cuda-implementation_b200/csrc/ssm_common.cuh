@@ -123,6 +123,14 @@ __device__ __forceinline__ float decay_rate(float a) {
     return r < -3.0e38f ? -3.0e38f : r;
 }
 
+// exp2(step * rate), the decays of one state over a step.  The hardware's exponential falls short of the value by 2e-8 on average for
+// exponents from -0.25 to -1e-3, and by 7e-9 nearer to 0 (measured): a state that lives for a thousand positions would collect
+// that a thousand times.  2e-8 in the exponent, added where it is multiplied anyway, takes the larger part of it back; a step of 0
+// is still a decay of exactly 1.  (The gradient of A at 4 x 4096 positions: 1.8e-6 off without, 8e-7 with it.)
+constexpr float DECAY_OFFSET = 2e-8f;
+__device__ __forceinline__ f2 decay2(f2 step, f2 rate) { return exp2_2(fma2(step, rate, splat2(DECAY_OFFSET))); }
+__device__ __forceinline__ float decay_f(float step, float rate) { return fast_exp2(fmaf(step, rate, DECAY_OFFSET)); }
+
 // values of a parameter of the lane's two channels
 __device__ __forceinline__ f2 param2(const float* p, int c, int n) { return pack2(p && n > 0 ? p[c] : 0.f, p && n > 1 ? p[c + 1] : 0.f); }
 
