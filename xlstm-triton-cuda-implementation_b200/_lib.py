@@ -192,11 +192,12 @@ def require_one_cuda_device(first, *others):
 
 
 _NO_GUARD = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def device_guard(dev):
     """``torch.cuda.device(dev)`` where another device is current, else nothing (the switch costs a few us a call)."""
-    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _NO_GUARD if _current_device() == dev.index else torch.cuda.device(dev)
 
 
 def ptr(t):

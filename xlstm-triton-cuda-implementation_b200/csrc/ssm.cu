@@ -242,10 +242,11 @@ __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArg
 
 template <typename T, int K, bool OUT>
 cudaError_t launch_ssm_fwd_pass(const SsmFwdArgs& a, int segs, cudaStream_t st) {
-    auto kern = a.pairs && a.N == K * SSM_WARPS ? ssm_fwd_kernel<T, K, OUT, true, true>
-                : a.pairs ? ssm_fwd_kernel<T, K, OUT, true, false> : ssm_fwd_kernel<T, K, OUT, false, false>;
     constexpr size_t smem = sizeof(SsmFwdSmem<K>);
-    const cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    static std::atomic<unsigned long long> done[3];
+    const int v = !a.pairs ? 0 : a.N == K * SSM_WARPS ? 2 : 1;
+    auto kern = v == 2 ? ssm_fwd_kernel<T, K, OUT, true, true> : v == 1 ? ssm_fwd_kernel<T, K, OUT, true, false> : ssm_fwd_kernel<T, K, OUT, false, false>;
+    const cudaError_t ce = ssm_allow_smem(kern, smem, done[v]);
     if (ce != cudaSuccess) return ce;
     return launch_plain(kern, dim3(static_cast<unsigned>(a.G * a.tiles_g), segs, a.Bt), dim3(SSM_THREADS), smem, st, a);
 }

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
 }
 
 template <typename T, int K, int W, bool GATED, bool PAIRS, bool FULL>
-__global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(const SsmBwdArgs p) {
+__global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
     constexpr int NP = K * W, IT = SSM_CK / W, SIT = BWD_ROWS / W > 0 ? BWD_ROWS / W : 1, BI = SSM_CK * NP / (32 * W) > 0 ? SSM_CK * NP / (32 * W) : 1, BSTEP = 32 * W / NP;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SsmBwdSmem<T, K, W>& sm = *reinterpret_cast<SsmBwdSmem<T, K, W>*>(smem_raw);
@@ -472,10 +472,13 @@ template <typename T, int K, int W>
 cudaError_t launch_ssm_bwd(SsmBwdArgs a, const SsmBwdWs& w, void* dB, void* dC, cudaStream_t st) {
     const unsigned tiles = static_cast<unsigned>(a.G * a.tiles_g);
     constexpr size_t smem = sizeof(SsmBwdSmem<T, K, W>);
-    const bool full = a.pairs && a.N == K * W;
-    auto kern = a.z ? (full ? ssm_bwd_kernel<T, K, W, true, true, true> : a.pairs ? ssm_bwd_kernel<T, K, W, true, true, false> : ssm_bwd_kernel<T, K, W, true, false, false>)
-                    : (full ? ssm_bwd_kernel<T, K, W, false, true, true> : a.pairs ? ssm_bwd_kernel<T, K, W, false, true, false> : ssm_bwd_kernel<T, K, W, false, false, false>);
-    cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    static std::atomic<unsigned long long> done[6];
+    const int v = (!a.pairs ? 0 : a.N == K * W ? 2 : 1) + (a.z ? 3 : 0);
+    void (*const kerns[6])(SsmBwdArgs) = {ssm_bwd_kernel<T, K, W, false, false, false>, ssm_bwd_kernel<T, K, W, false, true, false>,
+                                          ssm_bwd_kernel<T, K, W, false, true, true>,   ssm_bwd_kernel<T, K, W, true, false, false>,
+                                          ssm_bwd_kernel<T, K, W, true, true, false>,   ssm_bwd_kernel<T, K, W, true, true, true>};
+    auto kern = kerns[v];
+    cudaError_t ce = ssm_allow_smem(kern, smem, done[v]);
     for (int b0 = 0; b0 < a.Bt && ce == cudaSuccess; b0 += w.nb) {
         a.b0 = b0;
         a.nb = a.Bt - b0 < w.nb ? a.Bt - b0 : w.nb;

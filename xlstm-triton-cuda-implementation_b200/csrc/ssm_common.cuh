@@ -13,6 +13,7 @@
 // leave (the sum over the states, D x, the gate).  The two halves work on different tiles of positions at the same time, two
 // buffers each way, handed over by named barriers.
 #pragma once
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -154,6 +155,18 @@ int ssm_fill(SsmArgs& a, const void* x, const void* dt, const float* A, const vo
              const float* bias, const long long* strides, int Bt, int S, int Ch, int G, int N, int dtype, int softplus);
 void ssm_cut(SsmArgs& a, int ctas_per_sm);
 bool ssm_pairs(const SsmArgs& a, int es, std::initializer_list<const void*> more);
+// Lets a kernel have more shared memory than a plain launch, once for each device (a call of its own costs a microsecond on the host).
+template <typename... KArgs>
+inline cudaError_t ssm_allow_smem(void (*kern)(KArgs...), size_t bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t ce = cudaGetDevice(&dev);
+    if (ce != cudaSuccess) return ce;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (ce == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return ce;
+}
 inline bool ssm_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 }  // namespace mlstm

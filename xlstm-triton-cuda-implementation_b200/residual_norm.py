@@ -22,8 +22,8 @@ from . import _lib
 __all__ = ["residual_rms_norm", "residual_rms_norm_backward", "residual_rms_norm_quantized"]
 
 
-def _check(x, weight, residual):
-    """(device, rows, D, groups, inner) of x with this weight."""
+def _check(x, weight, residual, w_dtype=None):
+    """(device, rows, D, groups, inner) of x with this weight; ``w_dtype``: a type that the weight may have beside x's and float32."""
     if x.dim() < 1 or x.numel() == 0:
         raise ValueError("x must have at least one row of at least one value")
     D = x.shape[-1]
@@ -35,7 +35,7 @@ def _check(x, weight, residual):
             if x.dim() != 4 or weight.shape != (x.shape[1], D):
                 raise ValueError("weight must have the shape [D], or [NH, D] for x [B, NH, S, D]")
             groups, inner = x.shape[1], x.shape[2]
-        if weight.dtype not in (x.dtype, torch.float32):
+        if weight.dtype not in (x.dtype, torch.float32, w_dtype):
             raise TypeError("weight must have x's element type or float32")
     if residual is not None:
         if residual.shape != x.shape:
@@ -49,8 +49,8 @@ def _check(x, weight, residual):
     return dev, x.numel() // D, D, groups, inner
 
 
-def _forward(x, weight, residual, eps, out, scale, block):
-    dev, rows, D, groups, inner = _check(x, weight, residual)
+def _forward(checked, x, weight, residual, eps, out, scale, block):
+    dev, rows, D, groups, inner = checked
     total = None if residual is None else torch.empty_like(residual)
     stream = x if residual is None else residual
     with _lib.device_guard(dev):
@@ -66,13 +66,11 @@ def residual_rms_norm_backward(dy, s, weight=None, ds=None, eps=1e-6, x_dtype=No
     """Gradients (dx, dresidual, dweight): ``s`` is the sum (x where there was no residual), ``ds`` the gradient that the sum gets
     from its later uses or None.  dx has ``x_dtype`` (default: that of s) and dresidual the type of s; where these are the same
     type they are one tensor."""
-    dev, rows, D, groups, inner = _check(s, None, None)
-    if weight is not None:
-        if weight.shape != (D,):
-            if s.dim() != 4 or weight.shape != (s.shape[1], D):
-                raise ValueError("weight must have the shape [D], or [NH, D] for s [B, NH, S, D]")
-            groups, inner = s.shape[1], s.shape[2]
-        _lib.require_cuda(s, weight)
+    return _backward(_check(s, weight, None, x_dtype), dy, s, weight, ds, eps, x_dtype)
+
+
+def _backward(checked, dy, s, weight, ds, eps, x_dtype):
+    dev, rows, D, groups, inner = checked
     if dy.shape != s.shape or (dy.dtype != s.dtype and s.dtype != torch.float32):
         raise ValueError("dy must have the shape of s, and its element type unless that is float32")
     if ds is not None and (ds.shape != s.shape or ds.dtype != s.dtype):
@@ -95,8 +93,9 @@ def residual_rms_norm_backward(dy, s, weight=None, ds=None, eps=1e-6, x_dtype=No
 class _ResidualRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, out_dtype):
-        y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
-        total = _forward(x, weight, residual, eps, y, None, 0)
+        ctx.checked = _check(x, weight, residual)
+        y = torch.empty_like(x) if out_dtype is x.dtype else torch.empty_like(x, dtype=out_dtype)
+        total = _forward(ctx.checked, x, weight, residual, eps, y, None, 0)
         ctx.save_for_backward(x if total is None else total, weight)
         ctx.eps, ctx.x_dtype, ctx.with_residual = eps, x.dtype, residual is not None
         ctx.set_materialize_grads(False)
@@ -108,8 +107,8 @@ class _ResidualRmsNorm(torch.autograd.Function):
         s, weight = ctx.saved_tensors
         if dy is None:          # only the sum was used
             return (None if ds is None else ds.to(ctx.x_dtype)), None, ds, None, None
-        dx, dres, dweight = residual_rms_norm_backward(dy.contiguous(), s, weight, None if ds is None else ds.contiguous(), ctx.eps,
-                                                       ctx.x_dtype)
+        dx, dres, dweight = _backward(ctx.checked, dy.contiguous(), s, weight, None if ds is None else ds.contiguous(), ctx.eps,
+                                      ctx.x_dtype)
         return dx, dweight, dres if ctx.with_residual else None, None, None
 
 
@@ -120,8 +119,9 @@ def residual_rms_norm(x, weight=None, residual=None, eps=1e-6, out_dtype=None):
         raise TypeError("out_dtype must be the type of the stream (x, or the residual), or any where that is float32")
     if torch.is_grad_enabled() and any([t.requires_grad for t in (x, weight, residual) if t is not None]):
         return _ResidualRmsNorm.apply(x, weight, residual, float(eps), out_dtype)
-    y = torch.empty_like(x) if out_dtype is x.dtype and x.is_contiguous() else x.new_empty(x.shape, dtype=out_dtype)
-    total = _forward(x, weight, residual, float(eps), y, None, 0)
+    checked = _check(x, weight, residual)
+    y = torch.empty_like(x) if out_dtype is x.dtype else torch.empty_like(x, dtype=out_dtype)
+    total = _forward(checked, x, weight, residual, float(eps), y, None, 0)
     return y if total is None else (y, total)
 
 
@@ -135,7 +135,8 @@ def residual_rms_norm_quantized(x, weight=None, residual=None, eps=1e-6, block=N
     if block is not None and (block not in (32, 64, 128) or D % block):
         raise ValueError("block must be None (one scale per row), 32, 64 or 128, and divide the last dimension")
     block = D if block is None else block
+    checked = _check(x, weight, residual)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1] + (D // block if block else 0,), dtype=torch.float32, device=x.device)
-    total = _forward(x, weight, residual, float(eps), q, scale, block)
+    scale = torch.empty(x.shape[:-1] + (D // block,), dtype=torch.float32, device=x.device)
+    total = _forward(checked, x, weight, residual, float(eps), q, scale, block)
     return (q, scale) if total is None else (q, scale, total)

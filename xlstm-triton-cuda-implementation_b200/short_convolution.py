@@ -55,8 +55,8 @@ def _check(x, weight, bias, activation):
     return dev, _Strides(s[0], s[1])
 
 
-def _forward(x, weight, bias, activation, initial, state_out):
-    dev, strides = _check(x, weight, bias, activation)
+def _forward(checked, x, weight, bias, activation, initial=None, state_out=None):
+    dev, strides = checked
     B, S, C = x.shape
     W = weight.shape[1]
     for name, t in (("initial", initial), ("state_out", state_out)):
@@ -73,7 +73,11 @@ def _forward(x, weight, bias, activation, initial, state_out):
 
 def short_convolution_backward(dy, x, weight, bias=None, activation=None):
     """Gradients (dx, dweight, dbias) of ``short_convolution`` without states; dbias is None where there is no bias."""
-    dev, strides = _check(x, weight, bias, activation)
+    return _backward(_check(x, weight, bias, activation), dy, x, weight, bias, activation)
+
+
+def _backward(checked, dy, x, weight, bias, activation):
+    dev, strides = checked
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("dy must match x in shape and element type")
     _lib.require_cuda(dy, weight)
@@ -97,14 +101,13 @@ class _ShortConvolution(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation):
         ctx.save_for_backward(x, weight, bias)
-        ctx.activation = activation
-        return _forward(x, weight, bias, activation, None, None)
+        ctx.activation, ctx.checked = activation, _check(x, weight, bias, activation)
+        return _forward(ctx.checked, x, weight, bias, activation)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
-        return short_convolution_backward(dy.contiguous(), x, weight, bias, ctx.activation) + (None,)
+        return _backward(ctx.checked, dy.contiguous(), *ctx.saved_tensors, ctx.activation) + (None,)
 
 
 def short_convolution(x, weight, bias=None, activation=None, initial=None, return_state=False, state_out=None):
@@ -116,10 +119,9 @@ def short_convolution(x, weight, bias=None, activation=None, initial=None, retur
     if not return_state:
         if state_out is not None:
             raise ValueError("state_out needs return_state")
-        return _forward(x, weight, bias, activation, initial, None)
+        return _forward(_check(x, weight, bias, activation), x, weight, bias, activation, initial)
+    checked = _check(x, weight, bias, activation)
     if state_out is None:
-        if x.dim() != 3 or weight.dim() != 2:
-            raise ValueError("x must have the shape [B, S, C] and weight [C, W]")
         state_out = (torch.empty_like(initial) if initial is not None and initial.is_contiguous()
-                     else x.new_empty((x.shape[0], max(weight.shape[1] - 1, 0), x.shape[2])))
-    return _forward(x, weight, bias, activation, initial, state_out), state_out
+                     else x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2])))
+    return _forward(checked, x, weight, bias, activation, initial, state_out), state_out

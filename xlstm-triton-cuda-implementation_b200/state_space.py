@@ -168,9 +168,8 @@ def state_space_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=F
         if state_out is not None:
             raise ValueError("state_out needs return_state")
         return state_space_scan_forward(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial)[0]
+    checked = _check(x, dt, A, B, C, D, z, dt_bias)
     if state_out is None:
-        if x.dim() != 3 or A.dim() != 2:
-            raise ValueError("x must have the shape [batch, S, channels] and A [channels, N]")
         state_out = (torch.empty_like(initial) if initial is not None and initial.is_contiguous()
                      else torch.empty((x.shape[0], x.shape[2], A.shape[1]), dtype=torch.float32, device=x.device))
-    return state_space_scan_forward(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial, state_out)[0], state_out
+    return _forward(checked, x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial, state_out)[0], state_out
