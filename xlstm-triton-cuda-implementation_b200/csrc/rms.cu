@@ -43,6 +43,21 @@ __device__ __forceinline__ void load_weight(const RmsArgs& p, long long at, floa
     else to_floats<__nv_bfloat16, V>(load_vec<__nv_bfloat16, V>(static_cast<const __nv_bfloat16*>(p.weight) + at), w);
 }
 
+// V values in 8 bits, scaled so that the magnitude `top` (its bits; 0: a block of zeros) becomes 448
+template <int V>
+__device__ __forceinline__ void store_fp8(uint8_t* q, const float (&v)[V], unsigned top) {
+    const float inv = top == 0u ? 1.0f : __fdividef(448.0f, __uint_as_float(top));
+    if constexpr (V == 8) {
+        __nv_fp8x2_storage_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        *reinterpret_cast<uint2*>(q) = make_uint2(o[0] | (static_cast<unsigned>(o[1]) << 16), o[2] | (static_cast<unsigned>(o[3]) << 16));
+    } else {
+        *q = __nv_cvt_float_to_fp8(v[0] * inv, __NV_SATFINITE, __NV_E4M3);
+    }
+}
+
 // Sum of a pair over the threads of a row: `tpr` lanes of a warp, or the whole block.  Every thread gets it.
 template <bool WARP>
 __device__ __forceinline__ float2 row_sum(float2 v, float2* sm, int tpr) {
@@ -66,7 +81,7 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2* sm, int tpr) {
 
 // T: x, S: the stream (x's type where there is no residual).  A thread's values are V neighbouring ones, K times.
 template <typename T, typename S, int V, int K, bool WARP, bool QUANT>
-__global__ void __launch_bounds__(WARP ? 128 : 512) rms_fwd_kernel(const RmsArgs p) {
+__global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 8 : V == 8 && K == 2 ? 3 : 1) rms_fwd_kernel(const RmsArgs p) {
     __shared__ float2 sm[32];
     extern __shared__ unsigned amax[];      // QUANT: largest magnitude of every block of the row (as bits: NaN above all)
     grid_dep_wait();
@@ -151,20 +166,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) rms_fwd_kernel(const RmsArgs
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int e = (k * tpr + tid) * V;
-            if (e < D) {
-                const unsigned t = top[e / p.block];
-                const float inv = t == 0u ? 1.0f : __fdiv_rn(448.0f, __uint_as_float(t));
-                uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.D + e;
-                if constexpr (V == 8) {
-                    __nv_fp8x2_storage_t o[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        o[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[k][2 * j] * inv, v[k][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                    *reinterpret_cast<uint2*>(q) = make_uint2(o[0] | (static_cast<unsigned>(o[1]) << 16), o[2] | (static_cast<unsigned>(o[3]) << 16));
-                } else {
-                    *q = __nv_cvt_float_to_fp8(v[k][0] * inv, __NV_SATFINITE, __NV_E4M3);
-                }
-            }
+            if (e < D) store_fp8<V>(static_cast<uint8_t*>(p.q) + row * p.D + e, v[k], top[e / p.block]);
         }
     }
 }

@@ -318,24 +318,33 @@ __global__ void __launch_bounds__(STEP_THREADS) ssm_step_kernel(const SsmStepArg
         bias[o] = p.bias ? p.bias[mine[o]] : 0.f;
         skip[o] = p.D ? p.D[mine[o]] : 0.f;
     }
-    for (int b = blockIdx.y; b < p.Bt; b += gridDim.y) {
-        float h[CH][4];
+    float next[CH][4];                       // the states of the sequence after the one that is worked on, on their way
+    auto fetch = [&](int b) {
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             const float* H = p.initial + (static_cast<size_t>(b) * p.Ch + c[i]) * p.N + n0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) h[i][j] = 0.f;
+            for (int j = 0; j < 4; j++) next[i][j] = 0.f;
             if (p.initial && on[i]) {
                 if (VEC) {
                     const float4 v = *reinterpret_cast<const float4*>(H);
-                    h[i][0] = v.x; h[i][1] = v.y; h[i][2] = v.z; h[i][3] = v.w;
+                    next[i][0] = v.x; next[i][1] = v.y; next[i][2] = v.z; next[i][3] = v.w;
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        if (j < nn) h[i][j] = H[j];
+                        if (j < nn) next[i][j] = H[j];
                 }
             }
         }
+    };
+    fetch(blockIdx.y);
+    for (int b = blockIdx.y; b < p.Bt; b += gridDim.y) {
+        float h[CH][4];
+#pragma unroll
+        for (int i = 0; i < CH; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[i][j] = next[i][j];
+        if (b + static_cast<int>(gridDim.y) < p.Bt) fetch(b + gridDim.y);
         for (int t = 0; t < p.S; t++) {
             float x[OWN], d[OWN], gate[OWN];
 #pragma unroll
