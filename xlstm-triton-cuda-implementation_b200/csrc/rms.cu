@@ -6,8 +6,10 @@
 //     ds = r (u - s r^2 mean(u s)) + (what comes down the stream),   dw = sum over the rows of dy s r.
 // Everything between the loads and the stores is fp32.
 //
-// Bound by HBM: every row is read once and held in registers between the sum over it and its use.  A row belongs to one warp
-// or, when it is longer than a warp's registers, to one block.
+// Bound by HBM: every row is read once and held in registers between the sum over it and its use.  A row belongs to a few lanes of
+// a warp or, when it is longer than their registers, to a block.  Measured, bf16: 16384 x 4096 with residual forward 81 us (6.6 TB/s),
+// backward 95 us (5.6 TB/s); 8192 x 4096 to 8 bits 50 us (4.7 TB/s: the blocks' barriers); 262144 rows of 128 fp32 values to
+// 16 bits, forward and backward, 127 us.
 #include <cuda_fp8.h>
 
 #include "reduce_rows.cuh"

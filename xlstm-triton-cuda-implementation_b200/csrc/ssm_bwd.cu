@@ -5,13 +5,21 @@
 //     dC_t = sum_c e_t h_t          dB_t = sum_c delta_t x_t g_t          dA = sum_t delta_t g_t u_t
 //     dx_t = delta_t sum_n g_t B_t + D e_t        ddelta_t = x_t sum_n g_t B_t + sum_n A g_t u_t
 //     dz_t = dy_t (sum_n C_t h_t + D x_t) silu'(z_t),   ddt = ddelta * sigmoid(dt + bias) behind a softplus
-// The positions are walked from the last to the first in runs of SSM_CK: the states inside a run are computed again from the
-// state that the forward kept in front of it, first the one in front of the second half, then for one half of SSM_ROWS
-// positions at a time all of them, in registers, together with the exponentials that the way back needs again.
+// W warps share the N states, K each, and walk the positions from the last to the first in runs of SSM_CK.  The states inside a run are
+// computed again from the one that the forward kept in front of it: first the one in its middle, then for BWD_ROWS positions at a
+// time all of them, in registers, together with the exponentials that the way back needs again.  All warps prepare and finish
+// (delta, e, the sums over the states); the next run's inputs are on their way to shared memory meanwhile.
 //
 // The sums over the channels (dB, dC) run over a CTA's 64 channels by a transposing butterfly (half of the values change hands at
 // every step, so 8 values cost 9 shuffles instead of 40) and over the CTAs of a group in a second kernel; the sums over the
 // states run over the warps through shared memory.  No atomics: the same inputs give the same bits.
+//
+// What bounds it: latency.  255 registers allow eight warps per SM, and a warp's two recurrences, exponentials, broadcasts and
+// butterflies are chains: 24 instructions per state and position, issue slots 50 %, shared memory 55 %, exponentials 29 % busy.
+// Measured, bf16, 16 states: 4 x 4096 x 4096 1.79 ms (2.29 with the forward), 2 x 2048 x 4096 0.53 ms.  Tried and slower for the
+// first (forward + backward, ms): four positions at a time (163 registers, more states recomputed) 2.59; four more warps that
+// prepare and finish, as in the forward 2.86; the channel sums through shared memory 2.38; two states per warp and sixteen warps
+// per SM 2.64.
 #include "reduce_rows.cuh"
 #include "ssm_common.cuh"
 

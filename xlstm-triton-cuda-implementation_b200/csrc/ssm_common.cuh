@@ -7,11 +7,10 @@
 // Everything between the loads and the stores is fp32.
 //
 // Layout of the work: a CTA owns SSM_CH = 64 neighbouring channels of one group, a lane two of them, so that a position's
-// row of 16-bit values is one 128-byte access and every arithmetic instruction is one on a pair of floats (f32x2).  Four of its
-// warps do the recurrence, K of the N states each; four more prepare what these read (delta and delta x of 64 channels, and
-// B_t[n], C_t[n], which are the same for all channels, twice each as pairs for one 16-byte broadcast) and finish what they
-// leave (the sum over the states, D x, the gate).  The two halves work on different tiles of positions at the same time, two
-// buffers each way, handed over by named barriers.
+// row of 16-bit values is one 128-byte access and every arithmetic instruction is one on a pair of floats (f32x2); its warps share
+// the N states among them.  B_t[n] and C_t[n] are the same for all channels of a CTA: they lie in shared memory twice each, as
+// pairs, and come as one 16-byte broadcast.  Where the channels do not fill the chip the positions are cut into segments: a first
+// pass takes what every segment adds to the state, and the second one starts each segment from the sum of those in front of it.
 #pragma once
 #include <atomic>
 #include <initializer_list>
@@ -24,8 +23,8 @@ namespace mlstm {
 constexpr int SSM_CH = 64;          // channels per CTA
 constexpr int SSM_ROWS = 8;         // positions whose operands a warp holds in registers at a time
 constexpr int SSM_MAX_N = 64;       // states per channel
-constexpr int SSM_WARPS = 4;        // warps that do the recurrence
-constexpr int SSM_AIDES = 4;       // warps that prepare and finish
+constexpr int SSM_WARPS = 4;        // forward: warps that do the recurrence
+constexpr int SSM_AIDES = 4;        // forward: warps that prepare and finish
 constexpr int SSM_THREADS = 32 * (SSM_WARPS + SSM_AIDES);
 constexpr int SSM_CK = 16;          // positions between two states that the forward keeps for the backward
 
