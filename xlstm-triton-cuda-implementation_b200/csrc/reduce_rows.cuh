@@ -5,10 +5,11 @@
 
 namespace mlstm {
 
-constexpr int RR_COLS = 32, RR_GROUPS = 32;
+constexpr int RR_COLS = 32;
 
-// out(column, sum): stores one sum.  A block takes 32 columns; 32 groups of threads take every 32nd row.
-template <typename Out>
+// out(column, sum): stores one sum.  A block takes 32 columns; RR_GROUPS groups of threads take every RR_GROUPS-th row: 32 where there
+// are rows for them, 4 where there are few (2 rows of 73728 columns: 14 us with 32).
+template <int RR_GROUPS, typename Out>
 __global__ void __launch_bounds__(RR_COLS * RR_GROUPS) reduce_rows_kernel(const float* __restrict__ part, int rows, long long cols, Out out) {
     __shared__ float sm[RR_GROUPS][RR_COLS];
     grid_dep_wait();
@@ -38,8 +39,9 @@ __global__ void __launch_bounds__(RR_COLS * RR_GROUPS) reduce_rows_kernel(const 
 
 template <typename Out>
 cudaError_t launch_reduce_rows(const float* part, int rows, long long cols, const Out& out, cudaStream_t st) {
-    return launch_plain(reduce_rows_kernel<Out>, dim3(static_cast<unsigned>((cols + RR_COLS - 1) / RR_COLS)), dim3(RR_COLS * RR_GROUPS),
-                        0, st, part, rows, cols, out);
+    const dim3 grid(static_cast<unsigned>((cols + RR_COLS - 1) / RR_COLS));
+    if (rows > 32) return launch_plain(reduce_rows_kernel<32, Out>, grid, dim3(RR_COLS * 32), 0, st, part, rows, cols, out);
+    return launch_plain(reduce_rows_kernel<4, Out>, grid, dim3(RR_COLS * 4), 0, st, part, rows, cols, out);
 }
 
 // a value stored in one of the element types

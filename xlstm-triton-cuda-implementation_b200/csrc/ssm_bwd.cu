@@ -118,30 +118,46 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
         G[k] = 0;
     }
     const int tiles = ceil_div(t_end - t_begin, TILE);
-    for (int tile = tiles - 1; tile >= 0; tile--) {
+    Raw2<T> rdt[IT], rdy[IT], rz[IT];               // the next tile (the one in front), on its way
+    T rC[BI];
+    auto fetch = [&](int tile) {
         const int t0 = t_begin + tile * TILE;
-        __syncthreads();
 #pragma unroll
         for (int i = 0; i < IT; i++) {
-            const int r = warp + W * i, t = t0 + r, n = t < t_end ? ch.n : 0;
-            f2 d = delta2(to_float2<T>(load_raw2<PAIRS>(dtp + t * p.sdt.t, n)), bias, p.softplus);
-            const float2 dy = to_float2<T>(load_raw2<PAIRS>(dyp + static_cast<size_t>(t) * p.Ch, n));
-            f2 e = pack2(dy.x, dy.y);
-            if (zp) {
-                const float2 z = to_float2<T>(load_raw2<PAIRS>(zp + t * p.sz.t, n));
-                e = mul2(e, mul2(pack2(z.x, z.y), sigmoid2(pack2(z.x, z.y))));
-            }
-            if (t >= t_end) d = 0;
-            *reinterpret_cast<ulonglong2*>(&sm_d[r][lane]) = make_ulonglong2(d, e);
+            const int t = t0 + warp + W * i, n = t < t_end ? ch.n : 0;
+            rdt[i] = load_raw2<PAIRS>(dtp + t * p.sdt.t, n);
+            rdy[i] = load_raw2<PAIRS>(dyp + static_cast<size_t>(t) * p.Ch, n);
+            if (zp) rz[i] = load_raw2<PAIRS>(zp + t * p.sz.t, n);
         }
 #pragma unroll
         for (int i = 0; i < BI; i++) {
             const int x = threadIdx.x + i * 32 * W, t = t0 + x / NP, n = x % NP;
-            if (x < TILE * NP) {
-                const float c = n < p.N && t < t_end ? to_f32<T>(Cp[t * p.sC.t + n]) : 0.f;
-                sm_c[x / NP][n] = make_float2(c, c);
-            }
+            rC[i] = x < TILE * NP && n < p.N && t < t_end ? Cp[t * p.sC.t + n] : from_f32<T>(0.f);
         }
+    };
+    fetch(tiles - 1);
+    for (int tile = tiles - 1; tile >= 0; tile--) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const int r = warp + W * i;
+            f2 d = delta2(to_float2<T>(rdt[i]), bias, p.softplus);
+            const float2 dy = to_float2<T>(rdy[i]);
+            f2 e = pack2(dy.x, dy.y);
+            if (zp) {
+                const float2 z = to_float2<T>(rz[i]);
+                e = mul2(e, mul2(pack2(z.x, z.y), sigmoid2(pack2(z.x, z.y))));
+            }
+            if (t_begin + tile * TILE + r >= t_end) d = 0;
+            *reinterpret_cast<ulonglong2*>(&sm_d[r][lane]) = make_ulonglong2(d, e);
+        }
+#pragma unroll
+        for (int i = 0; i < BI; i++) {
+            const int x = threadIdx.x + i * 32 * W;
+            const float c = to_f32<T>(rC[i]);
+            if (x < TILE * NP) sm_c[x / NP][x % NP] = make_float2(c, c);
+        }
+        if (tile > 0) fetch(tile - 1);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; k++) {
