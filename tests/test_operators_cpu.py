@@ -104,3 +104,20 @@ def test_scratch_sizes(pkg):
     assert L.mlstm_rms_bwd_workspace(16384, 4096, 1, 1) <= 148 * 8 * 4096 * 4
     assert 0 < L.mlstm_rms_bwd_workspace(7, 100, 1, 1) <= 7 * 100 * 4
     assert L.mlstm_conv_bwd_workspace(4, 4096, 4096, 4, 2) <= 4 * 4096 // 64 * 5 * 4096 * 4
+
+
+def test_convolution_scratch_covers_every_access_width(pkg):
+    """The number of partial sums follows from the channels per thread, which follow from types, sizes and alignment: the query has
+    to cover them all.  A call checks its scratch before its first launch (which fails here: no device)."""
+    L = pkg._lib.lib()
+    # 4 channels per thread: 16 blocks across 2048 channels, runs of 32 positions in blocks of four, one partial row each
+    assert L.mlstm_conv_bwd_workspace(4, 4096, 2048, 4, 2) >= 4 * (4096 // (32 * 4)) * 5 * 2048 * 4
+    if torch.cuda.is_available():
+        pytest.skip("the calls would launch")
+    at = lambda a: ctypes.c_void_p(a)
+    for dt in (0, 2):
+        for B, S, C in ((4, 4096, 2048), (1, 2000, 512), (2, 8192, 1024), (3, 777, 1344), (16, 500, 96), (1, 16384, 4096), (8, 3000, 768)):
+            for base in (4096, 4100):                # all channels of a thread at once, or one by one
+                need = L.mlstm_conv_bwd_workspace(B, S, C, 4, dt)
+                rc = L.mlstm_conv_bwd(at(base), at(base), at(4096), None, None, at(base), at(4096), None, at(4096), need, B, S, C, 4, dt, dt, 1, None)
+                assert rc not in (0, -5), (dt, B, S, C, base, rc)

@@ -380,12 +380,11 @@ int conv_check(const void* x, const void* weight, int B, int S, int C, int W, in
     return MLSTM_OK;
 }
 
-// partial rows of the parameters' gradients, for whichever access width the pointers allow
-size_t conv_part_rows(int B, int S, int C) {
+// bytes of the partial sums of the parameters' gradients with V channels per thread
+size_t conv_part_bytes(int B, int S, int C, int W, int V) {
     ConvArgs a{};
     a.Bt = B; a.S = S; a.C = C;
-    const size_t wide = conv_grid(a, 2, true).grid.y, one = conv_grid(a, 1, true).grid.y;
-    return static_cast<size_t>(B) * (wide > one ? wide : one);
+    return static_cast<size_t>(B) * conv_grid(a, V, true).grid.y * (W + 1) * C * sizeof(float);
 }
 
 }  // namespace
@@ -419,7 +418,9 @@ int mlstm_conv_fwd(const void* x, const void* weight, const void* bias, const vo
 size_t mlstm_conv_bwd_workspace(int B, int S, int C, int W, int dtype) {
     const void* any = reinterpret_cast<const void*>(16);
     if (conv_check(any, any, B, S, C, W, dtype, dtype, nullptr) != MLSTM_OK) return 0;
-    return conv_part_rows(B, S, C) * (W + 1) * C * sizeof(float);
+    // whichever access width the pointers of the call will allow: the grid, and with it the number of partial sums, follows from it
+    const size_t wide = conv_part_bytes(B, S, C, W, dtype == MLSTM_DT_F32 ? CONV_BYTES / 4 : CONV_BYTES / 2), one = conv_part_bytes(B, S, C, W, 1);
+    return wide > one ? wide : one;
 }
 
 int mlstm_conv_bwd(const void* dy, const void* x, const void* weight, const void* bias, const long long* strides, void* dx,
@@ -433,7 +434,7 @@ int mlstm_conv_bwd(const void* dy, const void* x, const void* weight, const void
         if (!aligned(q, es)) return MLSTM_E_ALIGN;
     for (const void* q : {weight, bias, static_cast<const void*>(dweight), static_cast<const void*>(dbias)})
         if (!aligned(q, ws)) return MLSTM_E_ALIGN;
-    if (!workspace || workspace_bytes < mlstm_conv_bwd_workspace(B, S, C, W, dtype) || !aligned(workspace, 16)) return MLSTM_E_WORKSPACE;
+    if (!workspace || !aligned(workspace, 16)) return MLSTM_E_WORKSPACE;
     ConvArgs a{};
     a.x = x; a.weight = weight; a.bias = bias; a.dy = dy; a.dx = dx; a.part = static_cast<float*>(workspace);
     a.sxb = strides ? strides[0] : static_cast<long long>(S) * C;
@@ -441,6 +442,7 @@ int mlstm_conv_bwd(const void* dy, const void* x, const void* weight, const void
     a.Bt = B; a.S = S; a.C = C; a.wdt = w_dtype; a.wvec = aligned(weight, 16) && aligned(bias, 16); a.silu = silu;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int V = conv_vec(a, es);
+    if (workspace_bytes < conv_part_bytes(B, S, C, W, V)) return MLSTM_E_WORKSPACE;
     cudaError_t ce = launch_conv<true>(a, W, V, dtype, st);
     if (ce == cudaSuccess) {
         const int rows = B * static_cast<int>(conv_grid(a, V, true).grid.y);
