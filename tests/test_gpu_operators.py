@@ -611,6 +611,127 @@ def test_same_call_same_bits(pk):
         assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
 
 
+# ---------------------------------------------------------------------------------------------- places and sizes off the beaten track
+def shifted(t, by=1):
+    """The same values, contiguous, ``by`` elements off the start of their memory."""
+    flat = torch.empty(t.numel() + by, dtype=t.dtype, device="cuda")
+    flat[by:] = t.reshape(-1).cuda()
+    return flat[by:].view(t.shape)
+
+
+def test_unaligned_tensors_give_the_same(pk):
+    """Contiguous views into flat buffers, off by one element: the slower accesses, the same arithmetic, so the same bits (for
+    the norm, whose rows are summed in another order, the same to a few roundings)."""
+    x, w, b, init, dy = conv_inputs(BF16, 2, 70, 96, 4, True, True, 1)
+    for make in (cu, shifted):
+        t = [make(v).requires_grad_(True) for v in (x, w, b)]
+        y, s = (v.detach() for v in pk.short_convolution(*(v.detach() for v in t), "silu", initial=make(init), return_state=True))
+        g = torch.autograd.grad(pk.short_convolution(*t, "silu"), t, make(dy))
+        if make is cu:
+            want = (y, s, g[0])
+        else:
+            assert all(torch.equal(u, v) for u, v in zip((y, s, g[0]), want))
+    a, sp = scan_inputs(BF16, 2, 40, 64, 16, 1, 2, initial=True)
+    for S in (40, 3):
+        cut = {k: (v[:, :S].contiguous() if k in ("x", "dt", "B", "C", "z") else v) for k, v in a.items()}
+        one = pk.state_space_scan(**on_gpu(cut), dt_softplus=sp, return_state=True)
+        two = pk.state_space_scan(**{k: shifted(v) for k, v in cut.items()}, dt_softplus=sp, return_state=True)
+        assert all(torch.equal(u, v) for u, v in zip(one, two))
+    x, w, r = norm_inputs(BF16, BF16, "x", (9, 256), 3)
+    (y0, s0), (y1, s1) = pk.residual_rms_norm(cu(x), cu(w), residual=cu(r)), pk.residual_rms_norm(shifted(x), shifted(w), residual=shifted(r))
+    assert torch.equal(s0, s1)
+    off(y1, oo.norm(s0.cpu(), w)[0], oo.HALF_STEP[BF16], 32 * U * y0.cpu().double().abs(), "y")
+
+
+@pytest.mark.parametrize("S", [6, 90])
+def test_scan_padding(pk, S):
+    """dt = -inf behind a softplus, in front of, between and behind the tokens: what is left is the sequence without those
+    positions, and they get gradients of 0."""
+    a, _ = scan_inputs(F32, 1, S, 64, 16, 1, 21, initial=True)
+    keep = torch.rand(S, generator=gen(3)) < 0.6
+    keep[0] = keep[-1] = False
+    a["dt"][:, ~keep] = -float("inf")
+    y, state = pk.state_space_scan(**on_gpu(a), dt_softplus=True, return_state=True)
+    short = {k: (v[:, keep] if k in ("x", "dt", "B", "C", "z") else v) for k, v in a.items()}
+    want, end = oo.scan(**short, softplus=True)
+    ym, hm = scan_mag(short, True)
+    off(state, end, U, scan_loss(S, 16) * hm, "state")
+    off(y[:, keep.cuda()], want, U, scan_loss(S, 16) * ym, "y")
+    d = {k: cu(v).requires_grad_(True) for k, v in a.items() if k != "initial"}
+    got = dict(zip(d, torch.autograd.grad(pk.state_space_scan(**d, dt_softplus=True).square().sum(), list(d.values()))))
+    assert all(bool(torch.isfinite(g).all()) for g in got.values())
+    assert not got["dt"][:, ~keep.cuda()].any() and not got["B"][:, ~keep.cuda()].any()
+
+
+def test_saved_tensors_that_come_back_with_other_strides(pk):
+    """Hooks that move what the backward needs to the host and back (contiguous then, where slices were saved)."""
+    wide = torch.randn(2, 30, 192, generator=gen(1)).to(BF16).cuda().requires_grad_(True)
+    w = (torch.randn(64, 4, generator=gen(2)) * 0.5).to(BF16).cuda().requires_grad_(True)
+    a, sp = scan_inputs(BF16, 2, 30, 64, 16, 1, 4, gated=False)
+    rest = {k: cu(v) for k, v in a.items() if k not in ("x", "z", "dt") and v is not None}
+
+    def step():
+        x, dt, z = wide.split(64, -1)
+        x = pk.short_convolution(x, w, None, "silu")
+        y = pk.state_space_scan(x, dt, z=z, dt_softplus=sp, **rest)
+        y = pk.residual_rms_norm(y, w[:, 0].contiguous())
+        return torch.autograd.grad(y.float().square().sum() + x.float().sum(), (wide, w))
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_scan_gradients_in_groups_of_batch_entries(pk):
+    """More partial sums of dB, dC than are held at one time: the last group is what its batch entries give alone."""
+    b, S, ch, N = 34, 1024, 2048, 64
+    assert pk._lib.lib().mlstm_ssm_bwd_workspace(b, S, ch, 1, N) < b * (ch // 64) * S * N * 8
+    g = torch.Generator("cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    x, dt, z, dy = (r(b, S, ch).to(BF16) for _ in range(4))
+    B, C = (r(b, S, N).to(BF16) for _ in range(2))
+    A, D, bias = -torch.exp(r(ch, N)), r(ch), r(ch) - 2
+
+    def run(k):
+        y, kept = pk.state_space_scan_forward(x[-k:], dt[-k:], A, B[-k:], C[-k:], D, z[-k:], bias, True, keep=True)
+        got = pk.state_space_scan_backward(dy[-k:], kept, x[-k:], dt[-k:], A, B[-k:], C[-k:], D, z[-k:], bias, True)
+        return [y] + [got[i] for i in (0, 1, 3, 4, 6)]
+    for u, v in zip(run(b), run(8)):
+        assert torch.equal(u[-8:], v)
+
+
+def test_offsets_beyond_32_bits(pk):
+    """More than 2^31 values in a tensor: the last channels at the last positions are what they are alone."""
+    g = torch.Generator("cuda").manual_seed(7)
+    B, S, C = 2, 16640, 64640          # 2.15e9 values
+    assert B * S * C > 2 ** 31
+    x = torch.empty(B, S, C, dtype=BF16, device="cuda").normal_(generator=g)
+    w = (torch.randn(C, 4, device="cuda", generator=g) * 0.5).to(BF16)
+    y = pk.short_convolution(x, w, None, "silu")
+    cut = slice(C - 64, C)
+    assert torch.equal(y[:, :, cut], pk.short_convolution(x[:, :, cut], w[cut].contiguous(), None, "silu"))
+    dx, _, _ = pk.short_convolution_backward(x, x, w, None, "silu")
+    assert torch.equal(dx[:, :, cut], pk.short_convolution_backward(x[:, :, cut].contiguous(), x[:, :, cut], w[cut].contiguous(), None, "silu")[0])
+    del dx
+    A, bias = -torch.exp(torch.randn(C, 1, device="cuda", generator=g)), torch.full((C,), -2.0, device="cuda")
+    Bv, Cv = (torch.randn(B, S, 1, device="cuda", generator=g).to(BF16) for _ in range(2))
+    y, kept = pk.state_space_scan_forward(x, x, A, Bv, Cv, None, None, bias, True, keep=True)
+    xs = x[:, :, cut].contiguous()
+    ys, ks = pk.state_space_scan_forward(xs, xs, A[cut], Bv, Cv, None, None, bias[cut], True, keep=True)
+    # (the narrow call is cut into segments, the wide one is not: the same sums in another order)
+    torch.testing.assert_close(y[:, :, cut].float(), ys.float(), rtol=2 * 2.0 ** -8, atol=1e-3)
+    got = pk.state_space_scan_backward(x, kept, x, x, A, Bv, Cv, None, None, bias, True)
+    want = pk.state_space_scan_backward(xs, ks, xs, xs, A[cut], Bv, Cv, None, None, bias[cut], True)
+    for k in (0, 1):
+        torch.testing.assert_close(got[k][:, :, cut].float(), want[k].float(), rtol=2 * 2.0 ** -8, atol=2e-3)
+    torch.testing.assert_close(got[2][cut], want[2], rtol=1e-3, atol=1e-2)
+    del got, kept, y
+    rows = x.view(-1, 8080)
+    n = pk.residual_rms_norm(rows)
+    assert torch.equal(n[-3:], pk.residual_rms_norm(rows[-3:].clone()))
+    assert torch.equal(pk.residual_rms_norm_backward(rows, rows)[0][-3:], pk.residual_rms_norm_backward(rows[-3:].clone(), rows[-3:].clone())[0])
+
+
 def test_library_refusals(pk):
     L, one = pk._lib.lib(), torch.zeros(64, device="cuda").data_ptr()
     assert L.mlstm_conv_fwd(one, one, None, None, None, one + 1, None, 1, 1, 8, 4, 2, 2, 1, None) == -3

@@ -75,7 +75,7 @@ def _backward(checked, dy, s, weight, ds, eps, x_dtype):
         raise ValueError("dy must have the shape of s, and its element type unless that is float32")
     if ds is not None and (ds.shape != s.shape or ds.dtype != s.dtype):
         raise ValueError("ds must match s in shape and element type")
-    _lib.require_cuda(s, dy, *(() if ds is None else (ds,)))
+    _lib.require_cuda(s, dy, *(() if ds is None else (ds,)), *(() if weight is None else (weight,)))
     x_dtype = s.dtype if x_dtype is None else x_dtype
     dx = torch.empty(s.shape, dtype=x_dtype, device=dev)
     dres = dx if x_dtype == s.dtype else torch.empty_like(s)

@@ -101,13 +101,14 @@ class _ShortConvolution(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation):
         ctx.save_for_backward(x, weight, bias)
-        ctx.activation, ctx.checked = activation, _check(x, weight, bias, activation)
-        return _forward(ctx.checked, x, weight, bias, activation)
+        ctx.activation = activation
+        return _forward(_check(x, weight, bias, activation), x, weight, bias, activation)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _backward(ctx.checked, dy.contiguous(), *ctx.saved_tensors, ctx.activation) + (None,)
+        saved = ctx.saved_tensors       # (their strides may be others than the forward's: hooks may have moved them away and back)
+        return _backward(_check(*saved, ctx.activation), dy.contiguous(), *saved, ctx.activation) + (None,)
 
 
 def short_convolution(x, weight, bias=None, activation=None, initial=None, return_state=False, state_out=None):

@@ -14,7 +14,8 @@ D, dt_bias: [channels], float32; N <= 64.  D, z and dt_bias may be None.  y has 
 ``initial`` ([batch, channels, N] float32) continues an earlier call, ``return_state`` gives the state behind this one, and
 ``state_out`` names the tensor it is written to, which may be ``initial`` itself (a decoding loop in a CUDA graph keeps one
 buffer).  Up to 8 positions take a kernel for decoding, as ``mlstm_chunkwise`` does for its mixer.  A position with delta = 0
-(no ``dt_softplus``) leaves the state as it is: so a batch of different lengths is padded on the left.
+(dt = -inf with ``dt_softplus``) and a finite x leaves the state as it is and gets gradients of 0 for dt and B: so a batch of
+different lengths is padded, on either side.
 
 Inputs that require gradients get them (no states in that case): the forward then keeps the state in front of every 16
 positions (N / 16 float32 values per element of x) and the backward recomputes what lies between.
@@ -146,16 +147,16 @@ def _backward(checked, dy, checkpoints, x, dt, A, B, C, D, z, dt_bias, dt_softpl
 class _StateSpaceScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, dt_softplus):
-        checked = _check(x, dt, A, B, C, D, z, dt_bias)
-        y, kept = _forward(checked, x, dt, A, B, C, D, z, dt_bias, dt_softplus, keep=True)
+        y, kept = _forward(_check(x, dt, A, B, C, D, z, dt_bias), x, dt, A, B, C, D, z, dt_bias, dt_softplus, keep=True)
         ctx.save_for_backward(kept, x, dt, A, B, C, D, z, dt_bias)
-        ctx.checked, ctx.dt_softplus = checked, dt_softplus
+        ctx.dt_softplus = dt_softplus
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _backward(ctx.checked, dy.contiguous(), *ctx.saved_tensors, ctx.dt_softplus) + (None,)
+        kept, *saved = ctx.saved_tensors    # (their strides may be others than the forward's: hooks may have moved them away and back)
+        return _backward(_check(*saved), dy.contiguous(), kept, *saved, ctx.dt_softplus) + (None,)
 
 
 def state_space_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial=None, return_state=False,
