@@ -6,8 +6,10 @@
 //
 // Bound by HBM: x in and y out (forward), x and dy in and dx out (backward).  Neighbouring threads own neighbouring channels, 8 bytes
 // each, and walk down the positions, so an input is read once (and W - 1 more at the start of each run, mostly from L2).
-// Measured, 4 x 4096 x 4096 bf16, W = 4, silu: forward 52 us (5.2 TB/s), backward 105 us with the sums of the parameters (3.8 TB/s),
-// where 37 (forward 17) instructions per value and the two hardware functions of silu are next to the memory's time.
+// Measured, 4 x 4096 x 4096 bf16, W = 4, silu: forward 52 us (5.2 TB/s; the two hardware functions of silu 62 %, issue slots 69 % busy),
+// backward 98 us with the sums of the parameters (4.1 TB/s; 27 instructions per value, 55 % of the issue slots: three warps per
+// scheduler at 165 registers do not cover their latencies; four at 128 registers, where the form without silu spills: 100 us).
+#include "pair_math.cuh"
 #include "reduce_rows.cuh"
 #include "vec_cvt.cuh"
 
@@ -197,22 +199,30 @@ __global__ void __launch_bounds__(CONV_THREADS<false>, 3) conv_fwd_kernel(const 
     }
 }
 
-// Backward: the same walk over x and dy, and W - 1 positions further, whose d the run's last dx need.
+// Backward: the same walk over x and dy, and W - 1 positions further, whose d the run's last dx need.  Arithmetic on pairs of channels.
+template <int V>
+constexpr int PAIRS = (V + 1) / 2;      // (a single channel: a pair whose second half is idle)
+template <int V>
+__device__ __forceinline__ void pair_up(const float (&f)[V], f2 (&o)[PAIRS<V>]) {
+#pragma unroll
+    for (int j = 0; j < PAIRS<V>; j++) o[j] = pack2(f[2 * j], V > 1 ? f[V > 1 ? 2 * j + 1 : 0] : 0.f);
+}
+
 template <typename T, int V, int W, bool SILU>
-__global__ void __launch_bounds__(CONV_THREADS<true>, 4) conv_bwd_kernel(const ConvArgs p) {
-    constexpr int U = CONV_U, DEPTH = CONV_BWD_DEPTH;
-    __shared__ float red[CONV_THREADS<true>][V];
+__global__ void __launch_bounds__(CONV_THREADS<true>, 3) conv_bwd_kernel(const ConvArgs p) {
+    constexpr int U = CONV_U, DEPTH = CONV_BWD_DEPTH, P = PAIRS<V>;
+    __shared__ f2 red[CONV_THREADS<true>][P];
     __shared__ typename RowPipe<T, V, U, DEPTH, CONV_THREADS<true>>::Ring ring[2];
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
     grid_dep_wait();
     grid_dep_launch();
     const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V, b = blockIdx.z;
     const int t0 = (blockIdx.y * blockDim.y + threadIdx.y) * p.rows, n = min(p.S - t0, p.rows);
-    float dw[W + 1][V];            // dw[W]: the bias
+    f2 dw[W + 1][P];               // dw[W]: the bias
 #pragma unroll
     for (int k = 0; k <= W; k++)
 #pragma unroll
-        for (int j = 0; j < V; j++) dw[k][j] = 0.f;
+        for (int j = 0; j < P; j++) dw[k][j] = 0;
     if (c < p.C && n > 0) {
         const int have = p.S - t0, last = n + W - 1;             // positions from t0 on that there are; that are walked
         const T* x = static_cast<const T*>(p.x) + b * p.sxb + c;
@@ -229,60 +239,90 @@ __global__ void __launch_bounds__(CONV_THREADS<true>, 4) conv_bwd_kernel(const C
             }
             pipe_commit();
         }
-        float w[W][V], bias[V], v[W - 1 + U][V], d[W - 1 + U][V];
+        f2 w[W][P], bias[P], v[W - 1 + U][P], d[W - 1 + U][P];
+        {
+            float wf[W][V], bf[V];
+            load_weights<V, W>(p, c, wf, bf);
+            pair_up<V>(bf, bias);
+#pragma unroll
+            for (int k = 0; k < W; k++) pair_up<V>(wf[k], w[k]);
+        }
 #pragma unroll
         for (int k = 0; k < W - 1; k++) {
-            to_floats<T, V>(input_row<T, V, W>(p, x, b, t0 - (W - 1) + k, c), v[k]);
+            float f[V];
+            to_floats<T, V>(input_row<T, V, W>(p, x, b, t0 - (W - 1) + k, c), f);
+            pair_up<V>(f, v[k]);
 #pragma unroll
-            for (int j = 0; j < V; j++) d[k][j] = 0.f;
+            for (int j = 0; j < P; j++) d[k][j] = 0;
         }
-        load_weights<V, W>(p, c, w, bias);
+        const f2 one = pack2(1.f, 1.f), minus = pack2(-1.f, -1.f);
         for (int t = 0; t < last; t += U) {
             pipe_wait<AHEAD - 1>();
-            xs.take(v + (W - 1));
-            gs.take(d + (W - 1));
+            {
+                float f[U][V];
+                xs.take(f);
+#pragma unroll
+                for (int u = 0; u < U; u++) pair_up<V>(f[u], v[W - 1 + u]);
+                gs.take(f);
+#pragma unroll
+                for (int u = 0; u < U; u++) pair_up<V>(f[u], d[W - 1 + u]);
+            }
             if (t + AHEAD * U < last) {
                 xs.fetch(t + AHEAD * U, there);
                 gs.fetch(t + AHEAD * U, there);
             }
             pipe_commit();
+            // (a group in the middle of the run: no test between its positions, whose chains then overlap)
+            auto group = [&](auto whole) {
+                constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                float* g = d[W - 1 + u];
-                if (SILU) {
+                for (int u = 0; u < U; u++) {
+                    f2* g = d[W - 1 + u];
+                    if (SILU) {
 #pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        float a = bias[j];
+                        for (int j = 0; j < P; j++) {
+                            f2 a = bias[j];
 #pragma unroll
-                        for (int k = 0; k < W; k++) a = fmaf(w[k][j], v[u + k][j], a);
-                        const float sg = conv_sigmoid(a);
-                        g[j] *= sg * fmaf(a, 1.0f - sg, 1.0f);        // silu'
+                            for (int k = 0; k < W; k++) a = fma2(w[k][j], v[u + k][j], a);
+                            const f2 sg = sigmoid2(a);                    // silu' = sg (1 + a (1 - sg))
+                            g[j] = mul2(mul2(g[j], sg), fma2(a, fma2(sg, minus, one), one));
+                        }
                     }
                 }
-                if (t + u < n) {
 #pragma unroll
-                    for (int j = 0; j < V; j++) {
+                for (int u = 0; u < U; u++) {
+                    const f2* g = d[W - 1 + u];
+                    if (WHOLE || t + u < n) {
 #pragma unroll
-                        for (int k = 0; k < W; k++) dw[k][j] = fmaf(g[j], v[u + k][j], dw[k][j]);
-                        dw[W][j] += g[j];
+                        for (int j = 0; j < P; j++) {
+#pragma unroll
+                            for (int k = 0; k < W; k++) dw[k][j] = fma2(g[j], v[u + k][j], dw[k][j]);
+                            dw[W][j] = add2(dw[W][j], g[j]);
+                        }
+                    }
+                    if (WHOLE || (t + u >= W - 1 && t + u < last)) {      // dx_s = sum_k w[k] d_{s + (W - 1) - k}
+                        float out[V];
+#pragma unroll
+                        for (int j = 0; j < P; j++) {
+                            f2 a = mul2(w[0][j], d[W - 1 + u][j]);
+#pragma unroll
+                            for (int k = 1; k < W; k++) a = fma2(w[k][j], d[W - 1 + u - k][j], a);
+                            const float2 o = unpack2(a);
+                            out[2 * j] = o.x;
+                            if (V > 1) out[V > 1 ? 2 * j + 1 : 0] = o.y;
+                        }
+                        store_vec<T, V>(dx, from_floats<T, V>(out));
+                        dx += p.C;
                     }
                 }
-                if (t + u >= W - 1 && t + u < last) {        // dx_s = sum_k w[k] d_{s + (W - 1) - k}
-                    float out[V];
-#pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        out[j] = 0.f;
-#pragma unroll
-                        for (int k = 0; k < W; k++) out[j] = fmaf(w[k][j], d[W - 1 + u - k][j], out[j]);
-                    }
-                    *reinterpret_cast<Vec<T, V>*>(dx) = from_floats<T, V>(out);
-                    dx += p.C;
-                }
-            }
+            };
+            static_assert(U >= W - 1, "the first group alone has positions whose dx is another run's");
+            if (t > 0 && t + U <= n) group(std::true_type{});
+            else group(std::false_type{});
 #pragma unroll
             for (int k = 0; k < W - 1; k++)
 #pragma unroll
-                for (int j = 0; j < V; j++) {
+                for (int j = 0; j < P; j++) {
                     v[k][j] = v[U + k][j];
                     d[k][j] = d[U + k][j];
                 }
@@ -294,14 +334,19 @@ __global__ void __launch_bounds__(CONV_THREADS<true>, 4) conv_bwd_kernel(const C
     for (int k = 0; k <= W; k++) {
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < V; j++) red[tid][j] = dw[k][j];
+        for (int j = 0; j < P; j++) red[tid][j] = dw[k][j];
         __syncthreads();
         if (threadIdx.y == 0 && c < p.C) {
             for (int r = 1; r < static_cast<int>(blockDim.y); r++)
 #pragma unroll
-                for (int j = 0; j < V; j++) dw[k][j] += red[r * blockDim.x + threadIdx.x][j];
+                for (int j = 0; j < P; j++) dw[k][j] = add2(dw[k][j], red[r * blockDim.x + threadIdx.x][j]);
 #pragma unroll
-            for (int j = 0; j < V; j++) p.part[(row * (W + 1) + k) * p.C + c + j] = dw[k][j];
+            for (int j = 0; j < P; j++) {
+                const float2 o = unpack2(dw[k][j]);
+                float* part = p.part + (row * (W + 1) + k) * p.C + c + 2 * j;
+                part[0] = o.x;
+                if (V > 1) part[1] = o.y;
+            }
         }
     }
 }
