@@ -25,7 +25,7 @@ def scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, initial=N
     B, C = (t.repeat_interleave(ch // t.shape[2], 2) for t in (B, C))
     delta = dt if dt_bias is None else dt + dt_bias.double()
     if softplus:
-        delta = torch.clamp(delta, min=0) + torch.log1p(torch.exp(-delta.abs()))
+        delta = torch.logaddexp(delta, torch.zeros_like(delta))      # (its slope at 0 is 1/2, also by autograd)
     h = x.new_zeros(b, ch, A.shape[1]) if initial is None else initial.double()
     ys = []
     for t in range(S):

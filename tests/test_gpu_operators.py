@@ -226,6 +226,22 @@ def test_scan_gradients(pk, dtype, b, S, ch, N, G, softplus, skip, gated, bias, 
         off(gv, wv, oo.HALF_STEP[gv.dtype], loss * mag[n], "d" + n)
 
 
+def test_scan_gradients_where_softplus_bends(pk):
+    """dt of exactly 0 of either sign (slope 1/2), far out on both sides, and of -inf (slope 0)."""
+    a, _ = scan_inputs(F32, 2, 50, 70, 8, 1, 21, bias=False)
+    for at, v in ((0, 0.0), (7, -0.0), (16, 40.0), (17, -40.0), (30, -200.0), (49, -float("inf"))):
+        a["dt"][:, at] = v
+    dy = torch.randn(2, 50, 70, generator=gen(22))
+    names = [n for n in NAMES if a[n] is not None]
+    d = {k: None if v is None else v.requires_grad_(True) for k, v in on_gpu(a).items() if k != "initial"}
+    got = torch.autograd.grad(pk.state_space_scan(**d, dt_softplus=True), [d[n] for n in names], dy.cuda())
+    ref = {k: oo.leaf(v) for k, v in a.items() if k != "initial"}
+    want = torch.autograd.grad(oo.scan(**ref, softplus=True)[0], [ref[n] for n in names], dy.double())
+    mag = gradient_mag(a, dy, True)
+    for n, gv, wv in zip(names, got, want):
+        off(gv, wv, U, (2 * scan_loss(50, 8) + (2 * 50 + 2 + 70 / 64 + 64) * U) * mag[n], "d" + n)
+
+
 def gradient_mag(a, dy, softplus):
     """Every gradient's formula with all of its terms in absolute value."""
     a = {k: (None if v is None else v.detach().double()) for k, v in a.items()}
