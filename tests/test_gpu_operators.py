@@ -174,6 +174,13 @@ SCAN = [
     (BF16, 1, 97, 64, 64, 1, True, True, True, True, True, 0),
     (BF16, 1, 1500, 70, 16, 1, True, True, True, True, True, 0),    # cut into segments
     (F32, 1, 1111, 40, 50, 2, True, True, True, True, True, 0),
+    (BF16, 2, 90, 128, 24, 1, True, True, True, True, False, 0),    # 24 and 48 states, and numbers next to them
+    (F32, 1, 70, 66, 17, 1, True, True, True, True, False, 0),
+    (F16, 1, 1300, 64, 23, 2, True, True, True, True, False, 0),
+    (BF16, 1, 61, 65, 25, 1, True, True, True, True, False, 0),
+    (F32, 2, 66, 64, 48, 1, True, True, True, True, False, 0),
+    (BF16, 1, 1400, 64, 40, 1, True, True, True, True, False, 0),
+    (F16, 1, 40, 62, 49, 1, True, True, False, True, False, 0),
 ]
 
 

@@ -13,8 +13,9 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmlstm_b200.so")
-SOURCES = ["capi.cu", "chunk.cu", "chunk_pair.cu", "chunk_state.cu", "conv.cu", "gates.cu", "mm_simt.cu", "mm_tc.cu", "mm_tc_pair.cu", "rms.cu", "scan_gemm.cu", "selftest.cu",
-           "simt_gemm.cu", "ssm.cu", "ssm_bwd.cu", "step.cu"]
+# (the ones that take longest to compile first)
+SOURCES = ["ssm_bwd.cu", "ssm.cu", "capi.cu", "chunk.cu", "chunk_pair.cu", "chunk_state.cu", "conv.cu", "gates.cu", "mm_simt.cu", "mm_tc.cu", "mm_tc_pair.cu",
+           "rms.cu", "scan_gemm.cu", "selftest.cu", "simt_gemm.cu", "step.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -54,7 +55,7 @@ def build(force=False, verbose=False):
         if r.returncode != 0:
             raise RuntimeError("nvcc failed: " + " ".join(cmd))
 
-    with ThreadPoolExecutor(max_workers=4) as ex:
+    with ThreadPoolExecutor(max_workers=max(4, min(8, os.cpu_count() or 4))) as ex:
         list(ex.map(run, jobs))
     if jobs or not os.path.exists(LIB):
         run([nvcc, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a"])

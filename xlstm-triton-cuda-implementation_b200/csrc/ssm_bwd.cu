@@ -91,7 +91,7 @@ __device__ __forceinline__ float2 butterfly(float (&v)[R], float (&w)[R], int la
 // What one segment adds to the gradient of the state in front of it: G = exp(delta A) (G + C e), from the last position back.
 template <typename T, int K, int W, bool PAIRS>
 __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs p) {
-    constexpr int TILE = SSM_ROWS, NP = K * W, IT = TILE / W, BI = (TILE * NP) / (32 * W) > 0 ? (TILE * NP) / (32 * W) : 1;
+    constexpr int TILE = SSM_ROWS, NP = K * W, IT = TILE / W, BI = (TILE * NP + 32 * W - 1) / (32 * W);
     __shared__ float4 sm_d[TILE][32];       // delta, e
     __shared__ float2 sm_c[TILE][NP];       // C, C
     grid_dep_wait();
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(32 * W) ssm_back_state_kernel(const SsmBwdArgs
 
 template <typename T, int K, int W, bool GATED, bool PAIRS, bool FULL>
 __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
-    constexpr int NP = K * W, IT = SSM_CK / W, SIT = BWD_ROWS / W > 0 ? BWD_ROWS / W : 1, BI = SSM_CK * NP / (32 * W) > 0 ? SSM_CK * NP / (32 * W) : 1, BSTEP = 32 * W / NP;
+    constexpr int NP = K * W, IT = SSM_CK / W, SIT = BWD_ROWS / W > 0 ? BWD_ROWS / W : 1, BSTEP = 32 * W / NP, BI = (SSM_CK + BSTEP - 1) / BSTEP;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SsmBwdSmem<T, K, W>& sm = *reinterpret_cast<SsmBwdSmem<T, K, W>*>(smem_raw);
     grid_dep_wait();
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
     const T* zp = GATED ? static_cast<const T*>(p.z) + b * p.sz.b + (t_last + warp) * p.sz.t + ch.c : nullptr;
     const size_t row0 = static_cast<size_t>(b) * p.S;
     const T* dyp = static_cast<const T*>(p.dy) + (row0 + t_last + warp) * p.Ch + ch.c;
-    const int bt = threadIdx.x / NP, bn = threadIdx.x % NP;
+    const int bt = threadIdx.x < NP * BSTEP ? threadIdx.x / NP : SSM_CK, bn = threadIdx.x % NP;    // (SSM_CK: a thread with none)
     const T* Bp = static_cast<const T*>(p.B) + b * p.sB.b + (t_last + bt) * p.sB.t + static_cast<long long>(ch.g) * p.N + bn;
     const T* Cp = static_cast<const T*>(p.C) + b * p.sC.b + (t_last + bt) * p.sC.t + static_cast<long long>(ch.g) * p.N + bn;
     const float* kept = p.ckpt + ((static_cast<size_t>(b) * ceil_div(p.S, SSM_CK) + t_last / SSM_CK) * p.N + warp * K) * p.Cpad + ch.cp;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
                 }
             }
 #pragma unroll
-            for (int i = 0; i < (BWD_ROWS * NP + 32 * W - 1) / (32 * W); i++) {
+            for (int i = 0; i < (BWD_ROWS + BSTEP - 1) / BSTEP; i++) {
                 const int r = bt + BSTEP * i, t = tc + q + r;
                 if (r < BWD_ROWS && t < t_end && bn < p.N)
                     p.bc_part[((static_cast<size_t>(blockIdx.x) * p.nb + bl) * p.S + t) * p.N + bn] = sm.bcg[turn][r][bn];
@@ -515,12 +515,16 @@ cudaError_t launch_ssm_bwd(SsmBwdArgs a, const SsmBwdWs& w, void* dB, void* dC, 
     }
     return ce;
 }
+// (Three states per warp for 24 and six for 48: 901 and 1479 us for 2 x 2048 x 2048 positions and channels, bf16, forward included,
+// against 1014 and 1836 with four and eight, which leave the last two warps without any.)
 template <typename T>
 cudaError_t launch_ssm_bwd_n(const SsmBwdArgs& a, const SsmBwdWs& w, void* dB, void* dC, cudaStream_t st) {
     if (a.N <= 4) return launch_ssm_bwd<T, 1, 4>(a, w, dB, dC, st);
     if (a.N <= 8) return launch_ssm_bwd<T, 2, 4>(a, w, dB, dC, st);
     if (a.N <= 16) return ssm_bwd_wide(a) ? launch_ssm_bwd<T, 2, 8>(a, w, dB, dC, st) : launch_ssm_bwd<T, 4, 4>(a, w, dB, dC, st);
+    if (a.N <= 24) return launch_ssm_bwd<T, 3, 8>(a, w, dB, dC, st);
     if (a.N <= 32) return launch_ssm_bwd<T, 4, 8>(a, w, dB, dC, st);
+    if (a.N <= 48) return launch_ssm_bwd<T, 6, 8>(a, w, dB, dC, st);
     return launch_ssm_bwd<T, 8, 8>(a, w, dB, dC, st);
 }
 
