@@ -7,8 +7,8 @@
 // Bound by HBM: x in and y out (forward), x and dy in and dx out (backward).  Neighbouring threads own neighbouring channels, 8 bytes
 // each, and walk down the positions, so an input is read once (and W - 1 more at the start of each run, mostly from L2).
 // Measured, 4 x 4096 x 4096 bf16, W = 4, silu: forward 52 us (5.2 TB/s; the two hardware functions of silu 62 %, issue slots 69 % busy),
-// backward 98 us with the sums of the parameters (4.1 TB/s; 27 instructions per value, 55 % of the issue slots: three warps per
-// scheduler at 165 registers do not cover their latencies; four at 128 registers, where the form without silu spills: 100 us).
+// backward 97 us with the sums of the parameters (4.2 TB/s; 26 instructions per value, 54 % of the issue slots: three warps per
+// scheduler at 168 registers do not cover their latencies; four at 128 registers, where the form without silu spills: 100 us).
 #include "pair_math.cuh"
 #include "reduce_rows.cuh"
 #include "vec_cvt.cuh"
@@ -139,7 +139,8 @@ __device__ __forceinline__ void pipe_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void pipe_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-constexpr int CONV_U = 4, CONV_DEPTH = 4, CONV_BWD_DEPTH = 3;
+// (backward, with the forward's 52 us: groups of 3 rows 156, of 4 151, of 5 149, of 6 154, of 8 157 us)
+constexpr int CONV_U = 4, CONV_DEPTH = 4, CONV_BWD_U = 5, CONV_BWD_DEPTH = 3;
 
 // A thread walks down its run of positions with the last W inputs in registers.
 template <typename T, int V, int W, bool SILU>
@@ -210,7 +211,7 @@ __device__ __forceinline__ void pair_up(const float (&f)[V], f2 (&o)[PAIRS<V>]) 
 
 template <typename T, int V, int W, bool SILU>
 __global__ void __launch_bounds__(CONV_THREADS<true>, 3) conv_bwd_kernel(const ConvArgs p) {
-    constexpr int U = CONV_U, DEPTH = CONV_BWD_DEPTH, P = PAIRS<V>;
+    constexpr int U = CONV_BWD_U, DEPTH = CONV_BWD_DEPTH, P = PAIRS<V>;
     __shared__ f2 red[CONV_THREADS<true>][P];
     __shared__ typename RowPipe<T, V, U, DEPTH, CONV_THREADS<true>>::Ring ring[2];
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
