@@ -760,3 +760,30 @@ def test_library_refusals(pk):
     assert L.mlstm_conv_fwd(one, one, None, None, None, one + 1, None, 1, 1, 8, 4, 2, 2, 1, None) == -3
     assert L.mlstm_ssm_fwd(one, one, one, one, one, None, None, None, None, None, one, None, None, None, 0, 1, 4096, 8, 1, 4, 2, 1, None) == -5
     assert L.mlstm_rms_bwd(one, None, one, one, one, None, one, None, 0, 1, 8, 1, 1, 1e-6, 0, 0, 0, 0, None) == -5
+
+
+# ---------------------------------------------------------------------------------------------- 8 bits at the edges
+def eight_bits(y, block):
+    """(values, scales) of fp32 results by the definition; a quotient in fp32 is one in 64 bits, rounded (53 > 2 * 24 + 1)."""
+    v = y.cpu().double().reshape(-1, y.shape[-1] // block, block)
+    top = v.abs().amax(-1)
+    return v, torch.where(top > 0, top / 448, torch.ones_like(top)).float()
+
+
+def assert_eight_bits(q, scale, y, block):
+    v, want = eight_bits(y, block)
+    assert torch.equal(scale.cpu().reshape(want.shape), want)
+    nearest = (v / want.double()[..., None]).float().to(torch.float8_e4m3fn).float()
+    assert torch.equal(q.cpu().float().reshape(v.shape), nearest), int((q.cpu().float().reshape(v.shape) != nearest).sum())
+
+
+@pytest.mark.parametrize("shape,block", [((300, 4096), 128), ((90, 2048), None), ((999, 256), 32), ((64, 8200), None),
+                                         ((40, 777), None), ((3, 16384), 64)])
+def test_quantized_norm_to_the_nearest(pk, shape, block):
+    """Values of 16 bits, whose quotients by the scale lie on ties now and then: each goes where its quotient goes."""
+    x = (torch.randn(*shape, generator=gen(shape[0])) * 2).to(BF16)
+    res = torch.zeros(shape)
+    y = pk.residual_rms_norm(x.float().cuda())
+    for got in (pk.residual_rms_norm_quantized(x.cuda(), block=block), pk.residual_rms_norm_quantized(x.float().cuda(), block=block),
+                pk.residual_rms_norm_quantized(x.cuda(), residual=res.cuda(), block=block)):
+        assert_eight_bits(got[0], got[1], y, block or shape[-1])
