@@ -307,7 +307,8 @@ int mlstm_ssm_bwd(const void* dy, const void* x, const void* dt, const float* A,
  *   weight          of `w_dtype`, NULL (ones), or [groups, D]: row r takes weight row (r / inner) % groups, for [B, NH, S, D]
  *                   tensors groups = NH and inner = S; else groups = 1
  *   scale           NULL: y of `y_dtype` (any).  Else y is 8 bits (e4m3), scale [rows, D / block] float32 with block = 32, 64, 128 or
- *                   D (which divides D), each the largest magnitude of its block / 448 (1 for a block of zeros): y * scale is the
+ *                   D (which divides D), each the largest magnitude of its block / 448 (1 for a block of zeros, rounded up
+ *                   below the normal numbers): y, the nearest to the result / scale, times scale is the
  *                   result.  block = 0 without scale.
  * Backward: s is the sum (x where there was no residual) of `s_dtype`, dy of `dy_dtype` (s_dtype, or any where s_dtype is float32), ds
  * of `s_dtype` the gradient of the sum from its later uses or NULL; dx of `x_dtype`; dres of `s_dtype` or NULL (the same values as

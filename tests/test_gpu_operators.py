@@ -767,7 +767,10 @@ def eight_bits(y, block):
     """(values, scales) of fp32 results by the definition; a quotient in fp32 is one in 64 bits, rounded (53 > 2 * 24 + 1)."""
     v = y.cpu().double().reshape(-1, y.shape[-1] // block, block)
     top = v.abs().amax(-1)
-    return v, torch.where(top > 0, top / 448, torch.ones_like(top)).float()
+    exact = torch.where(top > 0, top / 448, torch.ones_like(top))
+    scale = exact.float()
+    up = (scale < 2.0 ** -126) & (scale.double() < exact)         # below the normal numbers: rounded up
+    return v, torch.where(up, scale + 2.0 ** -149, scale)
 
 
 def assert_eight_bits(q, scale, y, block):
@@ -787,3 +790,23 @@ def test_quantized_norm_to_the_nearest(pk, shape, block):
     for got in (pk.residual_rms_norm_quantized(x.cuda(), block=block), pk.residual_rms_norm_quantized(x.float().cuda(), block=block),
                 pk.residual_rms_norm_quantized(x.cuda(), residual=res.cuda(), block=block)):
         assert_eight_bits(got[0], got[1], y, block or shape[-1])
+
+
+@pytest.mark.parametrize("D,block", [(256, 64), (4096, 128), (96, None), (257, None)])
+def test_quantized_norm_of_tiny_and_huge_values(pk, D, block):
+    """Blocks whose largest magnitude has no finite reciprocal, or a scale below the normal numbers, beside ordinary ones."""
+    x = torch.randn(8, D, generator=gen(D))
+    x[0] *= 1e-40                        # (eps holds the root at 1e-3: results of 1e-37)
+    x[1] *= 1e-43
+    x[1, ::3] = 0
+    x[2] = 0
+    x[2, 5] = 2.0 ** -149                # the least of all numbers
+    x[3, : D // 2] *= 1e-37
+    x[4] = (x[4] * 3).round() * 2.0 ** -149
+    x[5] *= 1e-30
+    w = torch.ones(D)
+    for weight in (w, w * 0.1, w * 2e37):
+        y = pk.residual_rms_norm(x.cuda(), weight.cuda())
+        q, scale = pk.residual_rms_norm_quantized(x.cuda(), weight.cuda(), block=block)
+        assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(q.float()).all())
+        assert_eight_bits(q, scale, y, block or D)

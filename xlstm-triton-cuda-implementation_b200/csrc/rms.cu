@@ -59,11 +59,13 @@ __device__ __forceinline__ f2 quotient2(f2 a, f2 minus_b, f2 inv) {
 constexpr float FP8_MAX = 448.0f, FP8_TINY = 0x1p-80f;      // (remainders underflow where scales are below the latter)
 
 // The scale of a block of values from its largest magnitude (its bits).  A quotient by 448 is 1/14 of a unit away from where two numbers
-// are equally near, so this is the rounded one.
+// are equally near, so this is the rounded one.  Below the normal numbers it is rounded up: the scale of a block that is not all zeros
+// is not 0 then, and what is divided by it stays within 448.
 __device__ __forceinline__ float block_scale(unsigned top) {
     const float t = __uint_as_float(top);
     if (t >= FP8_TINY && top < 0x7f800000u) return quotient(t, FP8_MAX, 1.0f / FP8_MAX);
-    return top == 0u ? 1.0f : __fdiv_rn(t, FP8_MAX);
+    if (top == 0u) return 1.0f;
+    return t < FP8_MAX * 0x1p-126f ? __fdiv_ru(t, FP8_MAX) : __fdiv_rn(t, FP8_MAX);
 }
 
 // V values in 8 bits: each to the nearest of its quotient by the scale that is returned (of 16-bit inputs one in ten thousand lies on a

@@ -128,7 +128,8 @@ def residual_rms_norm(x, weight=None, residual=None, eps=1e-6, out_dtype=None):
 def residual_rms_norm_quantized(x, weight=None, residual=None, eps=1e-6, block=None):
     """(q, scale), with a residual (q, scale, s).  q: float8_e4m3fn, x's shape; scale: float32, x's shape with the last dimension
     D / block: the largest magnitude of a row, or of each ``block`` (32, 64, 128) of its values, divided by 448 (1 where all are
-    zero).  Values are the nearest to their quotients by that scale (ties to even); a block with an infinity or a NaN gets that as its scale."""
+    zero; rounded up below the normal numbers, so that the least of blocks has one that is not 0).  Values are the nearest to their
+    quotients by that scale (ties to even); a block with an infinity or a NaN gets that as its scale."""
     if torch.is_grad_enabled() and any([t.requires_grad for t in (x, weight, residual) if t is not None]):
         raise ValueError("the quantized norm has no gradients")
     D = x.shape[-1] if x.dim() else 0
