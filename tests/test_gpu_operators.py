@@ -810,3 +810,52 @@ def test_quantized_norm_of_tiny_and_huge_values(pk, D, block):
         q, scale = pk.residual_rms_norm_quantized(x.cuda(), weight.cuda(), block=block)
         assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(q.float()).all())
         assert_eight_bits(q, scale, y, block or D)
+
+
+# ---------------------------------------------------------------------------------------------- segments whose decay leaves the range
+def long_call(rate, step, S=3000):
+    """A narrow, long call (cut into segments) of 64 channels and 4 states, without a softplus."""
+    r = lambda *s: torch.randn(*s, generator=gen(31))
+    return dict(x=torch.zeros(1, S, 64), dt=torch.full((1, S, 64), step), A=torch.full((64, 4), rate), B=r(1, S, 4), C=r(1, S, 4), D=None, z=None,
+                dt_bias=None)
+
+
+def test_scan_segments_whose_decay_leaves_the_range(pk):
+    """A segment's decay may be more, or less, than a float holds: nothing grows to nothing, next to nothing to something, and
+    something is left of what is large, as position by position."""
+    S = 3000
+    assert pk._lib.lib().mlstm_ssm_fwd_workspace(1, S, 64, 1, 4) > 0
+    a = long_call(4.0, 1.0)
+    a["x"][:, -10:] = 1.0                              # e^40 behind them; e^192 over 48 positions in front
+    y, state = pk.state_space_scan(**on_gpu(a), return_state=True)
+    want, end = oo.scan(**a)
+    ym, hm = scan_mag(a, False)
+    off(state, end, U, scan_loss(S, 4) * hm, "state from nothing")
+    off(y, want, U, scan_loss(S, 4) * ym, "y from nothing")
+    for rate, before in ((2.0, 1e-36), (-2.0, 1e36)):
+        a = long_call(rate, 0.0)
+        a["dt"][:, :48] = 1.0                          # e^96, then nothing
+        a["initial"] = torch.full((1, 64, 4), before)
+        y, state = pk.state_space_scan(**on_gpu(a), return_state=True)
+        want, end = oo.scan(**a)
+        ym, hm = scan_mag(a, False)
+        off(state, end, U, scan_loss(S, 4) * hm, "state")
+        off(y, want, U, scan_loss(S, 4) * ym, "y")
+
+
+def test_scan_gradients_over_segments_whose_decay_leaves_the_range(pk):
+    """The same on the way back: where no gradient comes from behind, none grows out of it."""
+    S = 3000
+    a = long_call(4.0, 1.0)
+    a["dt"][:, :100] = 0.02
+    dy = torch.zeros(1, S, 64)
+    dy[:, :100] = torch.randn(1, 100, 64, generator=gen(1))
+    names = [n for n in NAMES if a[n] is not None]
+    d = {k: cu(v).requires_grad_(True) for k, v in a.items() if v is not None}
+    got = torch.autograd.grad(pk.state_space_scan(**d), [d[n] for n in names], dy.cuda())
+    ref = {k: oo.leaf(v) for k, v in a.items()}
+    want = torch.autograd.grad(oo.scan(**ref)[0], [ref[n] for n in names], dy.double())
+    mag = gradient_mag(a, dy, False)
+    assert float(want[0].abs().max()) > 0.1
+    for n, gv, wv in zip(names, got, want):
+        off(gv, wv, U, (2 * scan_loss(S, 4) + (2 * S + 1 + 64) * U) * mag[n], "d" + n)

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(SSM_THREADS, 2) ssm_fwd_kernel(const SsmFwdArg
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 const int n = warp * K + k;
-                if (n < p.N) h[k] = fma2(decay2(sum, rate[k]), h[k], *reinterpret_cast<const f2*>(seg_state(j, n)));
+                if (n < p.N) h[k] = carry2(sum, rate[k], h[k], *reinterpret_cast<const f2*>(seg_state(j, n)));
             }
         }
     }

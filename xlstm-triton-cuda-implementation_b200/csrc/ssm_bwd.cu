@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
         for (int k = 0; k < K; k++) {
             const int n = warp * K + k;
             if (n < p.N)
-                G[k] = fma2(decay2(sum, rate[k]), G[k], *reinterpret_cast<const f2*>(p.seg_end + (sj * p.N + n) * p.Cpad + ch.cp));
+                G[k] = carry2(sum, rate[k], G[k], *reinterpret_cast<const f2*>(p.seg_end + (sj * p.N + n) * p.Cpad + ch.cp));
         }
     }
 
