@@ -859,3 +859,24 @@ def test_scan_gradients_over_segments_whose_decay_leaves_the_range(pk):
     assert float(want[0].abs().max()) > 0.1
     for n, gv, wv in zip(names, got, want):
         off(gv, wv, U, (2 * scan_loss(S, 4) + (2 * S + 1 + 64) * U) * mag[n], "d" + n)
+
+
+# ---------------------------------------------------------------------------------------------- many groups
+def test_scan_of_many_groups(pk):
+    """More groups than a grid's second dimension has places, one channel each."""
+    G, S, N = 65537, 2, 1
+    g = gen(33)
+    r = lambda *s: torch.randn(*s, generator=g)
+    a = dict(x=r(1, S, G), dt=r(1, S, G), A=-torch.exp(r(G, N)), B=r(1, S, G, N), C=r(1, S, G, N), D=None, z=None, dt_bias=None)
+    dy = r(1, S, G)
+    names = [n for n in NAMES if a[n] is not None]
+    d = {k: cu(v).requires_grad_(True) for k, v in a.items() if v is not None}
+    y = pk.state_space_scan(**d, dt_softplus=True)
+    got = torch.autograd.grad(y, [d[n] for n in names], dy.cuda())
+    ref = {k: oo.leaf(v) for k, v in a.items()}
+    out = oo.scan(**ref, softplus=True)[0]
+    off(y, out, U, scan_loss(S, N) * scan_mag(a, True)[0], "y")
+    want = torch.autograd.grad(out, [ref[n] for n in names], dy.double())
+    mag = gradient_mag(a, dy, True)
+    for n, gv, wv in zip(names, got, want):
+        off(gv, wv, U, (2 * scan_loss(S, N) + (2 * S + 1 + 64) * U) * mag[n], "d" + n)

@@ -419,15 +419,15 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
     }
 }
 
-// dB, dC [Bt, S, G, N]: sums over the CTAs of a group.
+// dB, dC [Bt, S, G, N]: sums over the CTAs of a group, for the groups from g0 on.
 template <typename T>
 __global__ void __launch_bounds__(256) ssm_bc_sum_kernel(const float2* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC, int tiles_g,
-                                                         int G, int N, long long rows, long long row0) {
+                                                         int G, int g0, int N, long long rows, long long row0) {
     grid_dep_wait();
     grid_dep_launch();
     const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, per = rows * N;
     if (i >= per) return;
-    const int g = blockIdx.y;
+    const int g = g0 + blockIdx.y;
     const float2* q = part + static_cast<long long>(g) * tiles_g * per + i;
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll 8
@@ -509,9 +509,10 @@ cudaError_t launch_ssm_bwd(SsmBwdArgs a, const SsmBwdWs& w, void* dB, void* dC, 
         if (a.nseg > 1) ce = launch_plain(a.pairs ? ssm_back_state_kernel<T, K, W, true> : ssm_back_state_kernel<T, K, W, false>, dim3(tiles, a.nseg - 1, a.nb), dim3(32 * W), 0, st, a);
         if (ce == cudaSuccess) ce = launch_plain(kern, dim3(tiles, a.nseg, a.nb), dim3(32 * W), smem, st, a);
         const long long rows = static_cast<long long>(a.nb) * a.S;
-        if (ce == cudaSuccess)
-            ce = launch_plain(ssm_bc_sum_kernel<T>, dim3(static_cast<unsigned>((rows * a.N + 255) / 256), a.G), dim3(256), 0, st, a.bc_part,
-                              static_cast<T*>(dB), static_cast<T*>(dC), a.tiles_g, a.G, a.N, rows, static_cast<long long>(b0) * a.S);
+        constexpr int MOST = 65535;             // places of a grid's second dimension
+        for (int g0 = 0; g0 < a.G && ce == cudaSuccess; g0 += MOST)
+            ce = launch_plain(ssm_bc_sum_kernel<T>, dim3(static_cast<unsigned>((rows * a.N + 255) / 256), a.G - g0 < MOST ? a.G - g0 : MOST), dim3(256), 0, st,
+                              a.bc_part, static_cast<T*>(dB), static_cast<T*>(dC), a.tiles_g, a.G, g0, a.N, rows, static_cast<long long>(b0) * a.S);
     }
     return ce;
 }
