@@ -880,3 +880,18 @@ def test_scan_of_many_groups(pk):
     mag = gradient_mag(a, dy, True)
     for n, gv, wv in zip(names, got, want):
         off(gv, wv, U, (2 * scan_loss(S, N) + (2 * S + 1 + 64) * U) * mag[n], "d" + n)
+
+
+# ---------------------------------------------------------------------------------------------- padding beside decays of -inf
+def test_scan_gradients_of_padding_beside_decays_of_minus_infinity(pk):
+    a, _ = scan_inputs(F32, 2, 60, 64, 16, 1, 41)
+    a["A"][3, 2] = a["A"][10, 0] = -float("inf")
+    gap = torch.zeros(60, dtype=torch.bool)
+    gap[[0, 1, 17, 18, 33, 58, 59]] = True
+    a["dt"][:, gap] = -float("inf")
+    dy = 100 * torch.randn(2, 60, 64, generator=gen(42))
+    names = [n for n in NAMES if a[n] is not None]
+    d = {k: cu(v).requires_grad_(True) for k, v in a.items() if v is not None}
+    got = dict(zip(names, torch.autograd.grad(pk.state_space_scan(**d, dt_softplus=True), [d[n] for n in names], dy.cuda())))
+    assert all(bool(torch.isfinite(g).all()) for g in got.values())
+    assert not got["dt"][:, gap.cuda()].any() and not got["B"][:, gap.cuda()].any()

@@ -117,10 +117,11 @@ __device__ __forceinline__ f2 delta2(float2 raw, f2 bias, int softplus) {
     return softplus ? softplus2(unpack2(v)) : v;
 }
 
-// A in units of log2; -inf as the lowest finite value, so that a step of 0 leaves the state (0 * -inf would be NaN)
+// A in units of log2; -inf (and what is below -1e30) as -1e30: a step of 0 leaves the state (0 * -inf would be NaN), a step above 2e-28
+// nothing of it.  Nor does the gradient of such a step overflow, which behind a softplus of -inf is multiplied by a slope of 0.
 __device__ __forceinline__ float decay_rate(float a) {
     const float r = a * 1.44269504088896340736f;
-    return r < -3.0e38f ? -3.0e38f : r;
+    return r < -1.0e30f ? -1.0e30f : r;
 }
 
 // exp2(step * rate), the decays of one state over a step.  The hardware's exponential falls short of the value by 2e-8 on average for
