@@ -895,3 +895,22 @@ def test_scan_gradients_of_padding_beside_decays_of_minus_infinity(pk):
     got = dict(zip(names, torch.autograd.grad(pk.state_space_scan(**d, dt_softplus=True), [d[n] for n in names], dy.cuda())))
     assert all(bool(torch.isfinite(g).all()) for g in got.values())
     assert not got["dt"][:, gap.cuda()].any() and not got["B"][:, gap.cuda()].any()
+
+
+# ---------------------------------------------------------------------------------------------- values near the largest
+@pytest.mark.parametrize("S,C", [(1, 8), (3, 7), (3, 8), (70, 8)])
+@pytest.mark.parametrize("silu", [True, False])
+def test_convolution_gradient_behind_a_huge_last_input(pk, S, C, silu):
+    """What the walk adds up behind the last position may be beyond a float; it belongs to no output."""
+    x, dy = torch.randn(1, S, C, generator=gen(S)), torch.randn(1, S, C, generator=gen(2))
+    x[:, -1] = 3e38
+    w = torch.tensor([1.5, -1.25, 2.0, 0.5]).repeat(C, 1)          # half of it at the last position, twice of it behind
+    xc = x.cuda().requires_grad_(True)
+    got = torch.autograd.grad(pk.short_convolution(xc, w.cuda(), None, "silu" if silu else None), xc, dy.cuda())[0]
+    ref = oo.leaf(x)
+    want = torch.autograd.grad(oo.conv(ref, w, None, silu)[0], ref, dy.double())[0]
+    # as in test_convolution_gradients; the slope is exactly 1 where the last input counts
+    x[:, -1] = 0
+    pre, d = oo.conv(x.abs(), w.abs())[0], 1.1 * dy.double().abs()
+    fold = lambda t: oo.conv(t.flip(1), w.abs())[0].flip(1)
+    off(got, want, U, fold(d * (5 * U * pre * silu + 16 * U)) + 4 * U * fold(d), "dx")

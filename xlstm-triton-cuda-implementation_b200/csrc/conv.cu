@@ -290,6 +290,13 @@ __global__ void __launch_bounds__(CONV_THREADS<true>, 3) conv_bwd_kernel(const C
                         }
                     }
                 }
+                if (SILU && !WHOLE && t + U > there) {          // (what adds up behind the last position may be no number)
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int j = 0; j < P; j++)
+                            if (t + u >= there) d[W - 1 + u][j] = 0;
+                }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     const f2* g = d[W - 1 + u];
