@@ -914,3 +914,14 @@ def test_convolution_gradient_behind_a_huge_last_input(pk, S, C, silu):
     pre, d = oo.conv(x.abs(), w.abs())[0], 1.1 * dy.double().abs()
     fold = lambda t: oo.conv(t.flip(1), w.abs())[0].flip(1)
     off(got, want, U, fold(d * (5 * U * pre * silu + 16 * U)) + 4 * U * fold(d), "dx")
+
+
+# ---------------------------------------------------------------------------------------------- kernels that only large calls reach
+@pytest.mark.parametrize("dtype,b,S,ch,N,G,softplus,skip,gated,bias,initial,wide", [
+    (BF16, 38, 33, 256, 16, 1, True, True, True, True, False, 0), (F32, 38, 17, 255, 16, 1, True, True, False, True, False, 0),
+    (F16, 75, 40, 192, 11, 2, True, False, True, True, False, 0), (F32, 50, 24, 160, 9, 1, False, True, False, False, False, 0),
+    (BF16, 38, 7, 250, 16, 1, True, True, False, True, False, 2), (F16, 150, 50, 21, 13, 1, True, True, True, True, False, 0)])
+def test_scan_gradients_of_many_blocks(pk, dtype, b, S, ch, N, G, softplus, skip, gated, bias, initial, wide):
+    """9 to 16 states with more than 148 blocks of 64 channels: two blocks of four warps on each SM, in the place of one of eight."""
+    assert b * G * -(-ch // G // 64) > 148
+    test_scan_gradients(pk, dtype, b, S, ch, N, G, softplus, skip, gated, bias, initial, wide)
