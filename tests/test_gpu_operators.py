@@ -925,3 +925,26 @@ def test_scan_gradients_of_many_blocks(pk, dtype, b, S, ch, N, G, softplus, skip
     """9 to 16 states with more than 148 blocks of 64 channels: two blocks of four warps on each SM, in the place of one of eight."""
     assert b * G * -(-ch // G // 64) > 148
     test_scan_gradients(pk, dtype, b, S, ch, N, G, softplus, skip, gated, bias, initial, wide)
+
+
+@pytest.mark.parametrize("dtype,b,S,ch,N,G", [(BF16, 200, 1, 4096, 16, 1), (F32, 151, 3, 4096, 13, 2), (F16, 301, 2, 2048, 64, 1), (BF16, 700, 1, 1000, 4, 1),
+                                              (F32, 233, 1, 1037, 30, 1)])
+def test_scan_tokens_of_a_full_batch(pk, dtype, b, S, ch, N, G):
+    """More sequences than the blocks along them: each block takes several, an uneven share at the end, its states fetched ahead."""
+    g = torch.Generator("cuda").manual_seed(b)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    x, dt, z = (r(b, S, ch).to(dtype) for _ in range(3))
+    B, C = (r(b, S, G, N).to(dtype) for _ in range(2))
+    A, D, bias, first = -torch.exp(r(ch, N)), r(ch), r(ch) - 2, r(b, ch, N)
+    call = lambda at, **kw: pk.state_space_scan(x[at], dt[at], A, B[at], C[at], D, z[at], bias, True, initial=first[at], return_state=True, **kw)
+    y, state = call(slice(None))
+    alone = [call(slice(k, k + 1)) for k in range(b)]
+    assert torch.equal(y, torch.cat([v[0] for v in alone])) and torch.equal(state, torch.cat([v[1] for v in alone]))
+    a = dict(x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=bias, initial=first)
+    a = {k: v.cpu() for k, v in a.items()}
+    want, end = oo.scan(**a, softplus=True)
+    ym, hm = scan_mag(a, True)
+    off(state, end, U, scan_loss(S, N) * hm, "state")
+    off(y, want, oo.HALF_STEP[dtype], scan_loss(S, N) * ym, "y")
+    again, over = call(slice(None), state_out=first)          # over the states that come in
+    assert over is first and torch.equal(again, y) and torch.equal(first, state)
