@@ -948,3 +948,15 @@ def test_scan_tokens_of_a_full_batch(pk, dtype, b, S, ch, N, G):
     off(y, want, oo.HALF_STEP[dtype], scan_loss(S, N) * ym, "y")
     again, over = call(slice(None), state_out=first)          # over the states that come in
     assert over is first and torch.equal(again, y) and torch.equal(first, state)
+
+
+ALIGNED = [(dtype, 2, 333, C, W, bias, silu, False, w32, wide)
+           for dtype, C, w32 in ((BF16, 136, False), (BF16, 72, True), (F16, 64, False), (F16, 200, True), (F32, 66, False))
+           for W in (2, 3, 4) for silu, bias, wide in ((True, False, 0), (False, True, 0), (True, True, 8), (False, False, 16))]
+
+
+@pytest.mark.parametrize("dtype,B,S,C,W,bias,silu,initial,w32,wide", ALIGNED)
+def test_convolution_of_aligned_channels(pk, dtype, B, S, C, W, bias, silu, initial, w32, wide):
+    """Several channels per thread with every number of taps, with and without silu and bias, in both directions."""
+    test_convolution(pk, dtype, B, S, C, W, bias, silu, initial, w32, wide)
+    test_convolution_gradients(pk, dtype, B, S, C, W, bias, silu, initial, w32, wide)
