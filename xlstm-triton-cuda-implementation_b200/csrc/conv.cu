@@ -9,6 +9,7 @@
 // Measured, 4 x 4096 x 4096 bf16, W = 4, silu: forward 52 us (5.2 TB/s; the two hardware functions of silu 62 %, issue slots 69 % busy),
 // backward 97 us with the sums of the parameters (4.2 TB/s; 26 instructions per value, 54 % of the issue slots: three warps per
 // scheduler at 168 registers do not cover their latencies; four at 128 registers, where the form without silu spills: 100 us).
+#include "async_copy.cuh"
 #include "pair_math.cuh"
 #include "reduce_rows.cuh"
 #include "vec_cvt.cuh"
@@ -66,12 +67,6 @@ __device__ __forceinline__ void load_weights(const ConvArgs& p, int c, float (&w
         for (int k = 0; k < W; k++) w[k][j] = v[j * W + k];
     }
 }
-// sigmoid: two hardware functions, good to a few units in the last place (exp(-x) = inf gives 0)
-__device__ __forceinline__ float conv_sigmoid(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + fast_exp2(x * -1.44269504088896340736f)));
-    return y;
-}
 // row t of the inputs, t >= -(W - 1)
 template <typename T, int V, int W>
 __device__ __forceinline__ Vec<T, V> input_row(const ConvArgs& p, const T* x, int b, int t, int c) {
@@ -104,17 +99,14 @@ struct RowPipe {
     // row t + u of the run exists where t + u < n; else zeros
     __device__ __forceinline__ void fetch(int t, int n) {
         if constexpr (ASYNC) {
-            const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(&ring[slot_in * U][tid]));
+            const unsigned dst = shared_address(&ring[slot_in * U][tid]);
             constexpr unsigned pitch = THREADS * sizeof(Row);
             if (t + U <= n) {
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + u * pitch), "l"(next + u * stride), "n"(static_cast<int>(sizeof(Row))) : "memory");
+                for (int u = 0; u < U; u++) copy_async<sizeof(Row)>(dst + u * pitch, next + u * stride);
             } else {
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst + u * pitch), "l"(t + u < n ? next + u * stride : first),
-                                 "n"(static_cast<int>(sizeof(Row))), "r"(t + u < n ? static_cast<int>(sizeof(Row)) : 0) : "memory");
+                for (int u = 0; u < U; u++) copy_async_or_zeros<sizeof(Row)>(dst + u * pitch, t + u < n ? next + u * stride : first, t + u < n);
             }
             slot_in = slot_in + 1 == SLOTS ? 0 : slot_in + 1;
         } else {
@@ -135,10 +127,6 @@ struct RowPipe {
         if constexpr (ASYNC) slot_out = slot_out + 1 == SLOTS ? 0 : slot_out + 1;
     }
 };
-__device__ __forceinline__ void pipe_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void pipe_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // (backward, with the forward's 52 us: groups of 3 rows 156, of 4 151, of 5 149, of 6 154, of 8 157 us)
 constexpr int CONV_U = 4, CONV_DEPTH = 4, CONV_BWD_U = 5, CONV_BWD_DEPTH = 3;
 
@@ -158,17 +146,17 @@ __global__ void __launch_bounds__(CONV_THREADS<false>, 3) conv_fwd_kernel(const 
 #pragma unroll
     for (int g = 0; g < AHEAD; g++) {
         if (g * CONV_U < n) xs.fetch(g * CONV_U, n);
-        pipe_commit();
+        copies_commit();
     }
     float w[W][V], bias[V], v[W - 1 + CONV_U][V];
 #pragma unroll
     for (int k = 0; k < W - 1; k++) to_floats<T, V>(input_row<T, V, W>(p, x, b, t0 - (W - 1) + k, c), v[k]);
     load_weights<V, W>(p, c, w, bias);
     for (int t = 0; t < n; t += CONV_U) {
-        pipe_wait<AHEAD - 1>();
+        copies_wait<AHEAD - 1>();
         xs.take(v + (W - 1));
         if (t + AHEAD * CONV_U < n) xs.fetch(t + AHEAD * CONV_U, n);
-        pipe_commit();
+        copies_commit();
 #pragma unroll
         for (int u = 0; u < CONV_U; u++) {
             float out[V];
@@ -180,7 +168,7 @@ __global__ void __launch_bounds__(CONV_THREADS<false>, 3) conv_fwd_kernel(const 
             }
             if (SILU) {
 #pragma unroll
-                for (int j = 0; j < V; j++) out[j] *= conv_sigmoid(out[j]);
+                for (int j = 0; j < V; j++) out[j] *= sigmoid_f(out[j]);
             }
             if (t + u < n) *reinterpret_cast<Vec<T, V>*>(y) = from_floats<T, V>(out);
             y += p.C;
@@ -238,7 +226,7 @@ __global__ void __launch_bounds__(CONV_THREADS<true>, 3) conv_bwd_kernel(const C
                 xs.fetch(g * U, there);
                 gs.fetch(g * U, there);                              // (d = 0 behind the last position)
             }
-            pipe_commit();
+            copies_commit();
         }
         f2 w[W][P], bias[P], v[W - 1 + U][P], d[W - 1 + U][P];
         {
@@ -258,7 +246,7 @@ __global__ void __launch_bounds__(CONV_THREADS<true>, 3) conv_bwd_kernel(const C
         }
         const f2 one = pack2(1.f, 1.f), minus = pack2(-1.f, -1.f);
         for (int t = 0; t < last; t += U) {
-            pipe_wait<AHEAD - 1>();
+            copies_wait<AHEAD - 1>();
             {
                 float f[U][V];
                 xs.take(f);
@@ -272,7 +260,7 @@ __global__ void __launch_bounds__(CONV_THREADS<true>, 3) conv_bwd_kernel(const C
                 xs.fetch(t + AHEAD * U, there);
                 gs.fetch(t + AHEAD * U, there);
             }
-            pipe_commit();
+            copies_commit();
             // (a group in the middle of the run: no test between its positions, whose chains then overlap)
             auto group = [&](auto whole) {
                 constexpr bool WHOLE = decltype(whole)::value;
@@ -370,7 +358,6 @@ struct ConvParamOut {
 };
 
 inline long long ceil_up(long long a, long long b) { return (a + b - 1) / b; }
-inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // Bytes of a row that a thread takes where everything is aligned for that.  (16 bytes cost registers, and with them threads: 92 against
 // 68 us for 4 x 4096 x 4096 bf16 forward, before the copies were asynchronous; 4 bytes: 69.)

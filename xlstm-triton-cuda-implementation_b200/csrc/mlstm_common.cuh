@@ -158,6 +158,9 @@ inline cudaError_t launch_plain(void (*kern)(KArgs...), dim3 grid, dim3 block, s
     return launch_pdl<false>(kern, grid, block, smem, st, static_cast<Args&&>(args)...);
 }
 
+// (a: a power of two)
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
 // Remembers the last CUDA failure of this host thread for mlstm_last_error_detail(); returns MLSTM_E_CUDA.
 int note_cuda_error(cudaError_t err, const char* where);
 

@@ -12,6 +12,7 @@
 // 16 bits, forward and backward, 127 us.
 #include <cuda_fp8.h>
 
+#include "async_copy.cuh"
 #include "pair_math.cuh"
 #include "reduce_rows.cuh"
 #include "vec_cvt.cuh"
@@ -211,10 +212,6 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 8 : V == 8 && K == 2 
     }
 }
 
-__device__ __forceinline__ void copy16(void* shared, const void* global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(shared))), "l"(global) : "memory");
-}
-
 // S: the stream's type, T: dy's.  Blocks (or parts of warps) walk over the rows of one group and keep their part of the weight's
 // gradient.  Where a thread has eight values of a row (PIPE), its pieces of the next rows are on their way to shared memory
 // while it works on one (each thread reads back what it asked for itself: no barrier).
@@ -252,14 +249,14 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 4 : V == 8 && K == 1 
                 uint4* q = ring + stage * Pipe::PIECES * pitch;
 #pragma unroll
                 for (int c = 0; c < Pipe::NS; c++) {
-                    copy16(q + c * pitch, reinterpret_cast<const uint4*>(static_cast<const S*>(p.x) + at) + c);
-                    if (p.ds) copy16(q + (Pipe::NS + c) * pitch, reinterpret_cast<const uint4*>(static_cast<const S*>(p.ds) + at) + c);
+                    copy_async<16>(shared_address(q + c * pitch), reinterpret_cast<const uint4*>(static_cast<const S*>(p.x) + at) + c);
+                    if (p.ds) copy_async<16>(shared_address(q + (Pipe::NS + c) * pitch), reinterpret_cast<const uint4*>(static_cast<const S*>(p.ds) + at) + c);
                 }
 #pragma unroll
                 for (int c = 0; c < Pipe::NT; c++)
-                    copy16(q + (2 * Pipe::NS + c) * pitch, reinterpret_cast<const uint4*>(static_cast<const T*>(p.dy) + at) + c);
+                    copy_async<16>(shared_address(q + (2 * Pipe::NS + c) * pitch), reinterpret_cast<const uint4*>(static_cast<const T*>(p.dy) + at) + c);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            copies_commit();
         }
     };
     int stage = 0;
@@ -276,7 +273,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512, WARP ? 4 : V == 8 && K == 1 
         Vec<S, V> sv[K], dsv[K];
         Vec<T, V> dv[K];
         if constexpr (Pipe::ON) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(Pipe::STAGES - 2) : "memory");
+            copies_wait<Pipe::STAGES - 2>();
             const uint4* q = ring + stage * Pipe::PIECES * pitch;
 #pragma unroll
             for (int c = 0; c < Pipe::NS; c++) {
@@ -361,8 +358,6 @@ struct RmsWeightOut {
     AnyOut dw;
     __device__ __forceinline__ void operator()(long long at, float v) const { dw.put(at, v); }
 };
-
-inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 constexpr int RMS_MAX_D = 16384;
 // How a row is laid over threads: V values each, K times, by `lanes` lanes of a warp (several rows in a block of 128 threads) or, lanes

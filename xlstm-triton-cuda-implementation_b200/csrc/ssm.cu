@@ -561,11 +561,11 @@ int mlstm_ssm_fwd(const void* x, const void* dt, const float* A, const void* Bv,
     if (!y) return MLSTM_E_ARG;
     const int es = dtype == MLSTM_DT_F32 ? 4 : 2;
     for (const void* q : {x, dt, Bv, Cv, z, static_cast<const void*>(y)})
-        if (!ssm_aligned(q, es)) return MLSTM_E_ALIGN;
+        if (!aligned(q, es)) return MLSTM_E_ALIGN;
     for (const void* q : {static_cast<const void*>(A), static_cast<const void*>(D), static_cast<const void*>(dt_bias),
                           static_cast<const void*>(initial), static_cast<const void*>(state_out)})
-        if (!ssm_aligned(q, 4)) return MLSTM_E_ALIGN;
-    if (!ssm_aligned(checkpoints, 8)) return MLSTM_E_ALIGN;
+        if (!aligned(q, 4)) return MLSTM_E_ALIGN;
+    if (!aligned(checkpoints, 8)) return MLSTM_E_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t ce;
     if (S <= STEP_TOKENS && !checkpoints) {
@@ -574,8 +574,8 @@ int mlstm_ssm_fwd(const void* x, const void* dt, const float* A, const void* Bv,
         a.initial = initial; a.y = y; a.state_out = state_out;
         // whole pieces of four states, and of four values of B and C; four channels of one group
         const long long strides4 = a.sB.b | a.sB.t | a.sC.b | a.sC.t;
-        const bool vec = N % 4 == 0 && a.P % STEP_CH == 0 && (strides4 & 3) == 0 && ssm_aligned(A, 16) && ssm_aligned(initial, 16) &&
-                         ssm_aligned(state_out, 16) && ssm_aligned(Bv, 4 * es) && ssm_aligned(Cv, 4 * es);
+        const bool vec = N % 4 == 0 && a.P % STEP_CH == 0 && (strides4 & 3) == 0 && aligned(A, 16) && aligned(initial, 16) &&
+                         aligned(state_out, 16) && aligned(Bv, 4 * es) && aligned(Cv, 4 * es);
         ce = dtype == MLSTM_DT_F32 ? launch_ssm_step<float>(a, vec, st)
              : dtype == MLSTM_DT_F16 ? launch_ssm_step<__half>(a, vec, st) : launch_ssm_step<__nv_bfloat16>(a, vec, st);
     } else {
@@ -583,7 +583,7 @@ int mlstm_ssm_fwd(const void* x, const void* dt, const float* A, const void* Bv,
         static_cast<SsmArgs&>(a) = base;
         ssm_cut(a, SSM_FWD_CTAS);
         const SsmWs w = ssm_carve(workspace, a);
-        if (w.bytes && (!workspace || workspace_bytes < w.bytes || !ssm_aligned(workspace, 16))) return MLSTM_E_WORKSPACE;
+        if (w.bytes && (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 16))) return MLSTM_E_WORKSPACE;
         a.seg_end = w.seg_end; a.seg_sum = w.seg_sum;
         a.ckpt = checkpoints; a.initial = initial; a.y = y; a.state_out = state_out;
         a.pairs = ssm_pairs(a, es, {y});

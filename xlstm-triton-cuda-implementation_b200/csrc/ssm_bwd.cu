@@ -20,6 +20,7 @@
 // first (forward + backward, ms): four positions at a time (163 registers, more states recomputed) 2.59; four more warps that
 // prepare and finish, as in the forward 2.86; the channel sums through shared memory 2.38; two states per warp and sixteen warps
 // per SM 2.64.
+#include "async_copy.cuh"
 #include "reduce_rows.cuh"
 #include "ssm_common.cuh"
 
@@ -50,15 +51,11 @@ struct SsmBwdSmem {
     float2 h0[2][K * W][32];                // the states in front of the run
 };
 
-__device__ __forceinline__ void copy_async8(void* shared, const void* global) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(shared))), "l"(global) : "memory");
-}
 // a pair of channels to shared memory: asynchronously where it is one aligned access
 template <bool PAIRS, typename T>
 __device__ __forceinline__ void copy_raw2(Raw2<T>* shared, const T* global, int n) {
     if constexpr (PAIRS) {
-        constexpr int bytes = 2 * sizeof(T);
-        if (n) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(shared))), "l"(global), "n"(bytes) : "memory");
+        if (n) copy_async<2 * sizeof(T)>(shared_address(shared), global);
         else *shared = Raw2<T>{};
     } else {
         *shared = load_raw2<false>(global, n);
@@ -248,9 +245,9 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
         if (GATED) zp -= SSM_CK * p.sz.t;
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (warp * K + k < p.N) copy_async8(&sm.h0[buf][warp * K + k][lane], kept + static_cast<size_t>(k) * p.Cpad);
+            if (warp * K + k < p.N) copy_async<8>(shared_address(&sm.h0[buf][warp * K + k][lane]), kept + static_cast<size_t>(k) * p.Cpad);
         kept -= static_cast<size_t>(p.N) * p.Cpad;
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        copies_commit();
 #pragma unroll
         for (int i = 0; i < BI; i++) {
             const bool in = bn < p.N && bt + BSTEP * i < min(left, SSM_CK);
@@ -263,7 +260,7 @@ __global__ void __launch_bounds__(32 * W) ssm_bwd_kernel(SsmBwdArgs p) {
     fetch(t_end - t_last, (chunks - 1) & 1);
     for (int chunk = chunks - 1; chunk >= 0; chunk--) {
         const int tc = t_begin + chunk * SSM_CK, subs = ceil_div(min(SSM_CK, t_end - tc), BWD_ROWS), buf = chunk & 1;
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        copies_wait<0>();
         // (the run behind this one has been read: its last barrier lies in front of everything that is written here)
 #pragma unroll
         for (int i = 0; i < IT; i++) {
@@ -558,13 +555,13 @@ int mlstm_ssm_bwd(const void* dy, const void* x, const void* dt, const float* A,
     const int es = dtype == MLSTM_DT_F32 ? 4 : 2;
     for (const void* q : {dy, x, dt, Bv, Cv, z, static_cast<const void*>(dx), static_cast<const void*>(ddt), static_cast<const void*>(dB),
                           static_cast<const void*>(dC), static_cast<const void*>(dz)})
-        if (!ssm_aligned(q, es)) return MLSTM_E_ALIGN;
+        if (!aligned(q, es)) return MLSTM_E_ALIGN;
     for (const float* q : {A, D, dt_bias, static_cast<const float*>(dA), static_cast<const float*>(dD), static_cast<const float*>(d_dt_bias)})
-        if (!ssm_aligned(q, 4)) return MLSTM_E_ALIGN;
-    if (!ssm_aligned(checkpoints, 8)) return MLSTM_E_ALIGN;
+        if (!aligned(q, 4)) return MLSTM_E_ALIGN;
+    if (!aligned(checkpoints, 8)) return MLSTM_E_ALIGN;
     ssm_bwd_cut(a);
     const SsmBwdWs w = ssm_bwd_carve(workspace, a);
-    if (!workspace || workspace_bytes < w.bytes || !ssm_aligned(workspace, 16)) return MLSTM_E_WORKSPACE;
+    if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 16)) return MLSTM_E_WORKSPACE;
     a.seg_end = w.seg_end; a.seg_sum = w.seg_sum; a.param_part = w.param; a.bc_part = w.bc;
     a.ckpt = const_cast<float*>(checkpoints);
     a.dy = dy; a.dx = dx; a.ddt = ddt; a.dz = dz;

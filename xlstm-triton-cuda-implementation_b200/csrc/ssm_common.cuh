@@ -179,6 +179,5 @@ inline cudaError_t ssm_allow_smem(void (*kern)(KArgs...), size_t bytes, std::ato
     if (ce == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return ce;
 }
-inline bool ssm_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 }  // namespace mlstm
