@@ -266,6 +266,7 @@ int mlstm_chunk_sp_apply(const void* q, const void* k, const void* v, const void
  * Short causal convolution, channel by channel: y_t = act(bias + sum_k weight[c][k] x_{t-(W-1)+k}), W = 2, 3 or 4, act = silu or
  * none.  x [B,S,C] with element strides {batch, position} in `strides` (a host array; NULL: contiguous), y [B,S,C] contiguous;
  * weight [C,W] and bias [C] (or NULL) of `w_dtype`: the inputs' type or float32.
+ * B <= 65535, S <= 2^23, C <= 2^24.
  *   initial [B,W-1,C]    the inputs in front of position 0, or NULL (zeros)
  *   state_out [B,W-1,C]  the last W-1 inputs of the call (and of `initial` where S < W-1), or NULL; may be `initial` itself
  * Backward (of a call with no `initial`): dy, dx [B,S,C] contiguous, dweight, dbias of `w_dtype` (dbias NULL as bias is). */
@@ -282,7 +283,7 @@ int mlstm_conv_bwd(const void* dy, const void* x, const void* weight, const void
  *   y_t     = (sum_n Cv_t[g][n] h_t[n] + D[c] x_t) * silu(z_t)
  * x, dt, z [B,S,C], Bv, Cv [B,S,G,N] of `dtype`, the last (two) dimension(s) contiguous; `strides` (host, NULL: contiguous):
  * element strides {batch, position} of x, dt, Bv, Cv, z.  A [C,N], D [C], dt_bias [C] float32; D, z, dt_bias may be NULL.
- * y [B,S,C] contiguous.  States [B,C,N] float32: `initial` (NULL: zeros), `state_out` (NULL: not wanted; may be `initial`).
+ * B <= 65535, C <= 2^24, S < 2^31 - 32.  y [B,S,C] contiguous.  States [B,C,N] float32: `initial` (NULL: zeros), `state_out` (NULL: not wanted; may be `initial`).
  *   checkpoints   NULL, or mlstm_ssm_checkpoint_floats() floats that the backward of the same call takes
  * Up to mlstm_ssm_step_max_tokens() positions without checkpoints take a kernel of their own (decoding).
  * Backward (of a call with no `initial`): dy and dx, ddt, dz [B,S,C], dB, dC [B,S,G,N] contiguous of `dtype`; dA, dD, d_dt_bias
@@ -302,7 +303,7 @@ int mlstm_ssm_bwd(const void* dy, const void* x, const void* dt, const float* A,
                   int B, int S, int C, int G, int N, int dtype, int softplus, void* stream);
 
 /* Root-mean-square norm with the residual's addition: sum = x + residual, rounded to `s_dtype`; y = sum / sqrt(mean(sum^2) + eps)
- * * weight over the last dimension D <= 16384 of `rows` contiguous rows.
+ * * weight over the last dimension D <= 16384 of `rows` < 2^31 contiguous rows.
  *   residual, sum   of `s_dtype` (the type of x, or float32), both or neither (then s_dtype = dtype)
  *   weight          of `w_dtype`, NULL (ones), or [groups, D]: row r takes weight row (r / inner) % groups, for [B, NH, S, D]
  *                   tensors groups = NH and inner = S; else groups = 1

@@ -7,8 +7,9 @@
 // Bound by HBM: x in and y out (forward), x and dy in and dx out (backward).  Neighbouring threads own neighbouring channels, 8 bytes
 // each, and walk down the positions, so an input is read once (and W - 1 more at the start of each run, mostly from L2).
 // Measured, 4 x 4096 x 4096 bf16, W = 4, silu: forward 52 us (5.2 TB/s; the two hardware functions of silu 62 %, issue slots 69 % busy),
-// backward 97 us with the sums of the parameters (4.2 TB/s; 26 instructions per value, 54 % of the issue slots: three warps per
-// scheduler at 168 registers do not cover their latencies; four at 128 registers, where the form without silu spills: 100 us).
+// backward 99 us with the sums of the parameters (151 in all; 4.1 TB/s; 26 instructions per value, 54 % of the issue slots: three warps
+// per scheduler at 168 registers do not cover their latencies; four at 128 registers, where the form without silu spills: 3 us more).
+// One channel per thread, where widths, strides or addresses allow no more (4 x 4096 x 4095): forward 87, backward 205 us.
 #include "async_copy.cuh"
 #include "pair_math.cuh"
 #include "reduce_rows.cuh"
@@ -127,7 +128,8 @@ struct RowPipe {
         if constexpr (ASYNC) slot_out = slot_out + 1 == SLOTS ? 0 : slot_out + 1;
     }
 };
-// (backward, with the forward's 52 us: groups of 3 rows 156, of 4 151, of 5 149, of 6 154, of 8 157 us)
+// (backward, with the forward's 52 us: groups of 3 rows 156, of 4 151, of 5 149, of 6 154, of 8 157 us; all before the values behind the
+// last position were set to 0, which takes 1.5 us)
 constexpr int CONV_U = 4, CONV_DEPTH = 4, CONV_BWD_U = 5, CONV_BWD_DEPTH = 3;
 
 // A thread walks down its run of positions with the last W inputs in registers.

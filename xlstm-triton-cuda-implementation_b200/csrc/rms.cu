@@ -7,9 +7,14 @@
 // Everything between the loads and the stores is fp32.
 //
 // Bound by HBM: every row is read once and held in registers between the sum over it and its use.  A row belongs to a few lanes of
-// a warp or, when it is longer than their registers, to a block.  Measured, bf16: 16384 x 4096 with residual forward 81 us (6.6 TB/s),
-// backward 95 us (5.6 TB/s); 8192 x 4096 to 8 bits 50 us (4.7 TB/s: the blocks' barriers); 262144 rows of 128 fp32 values to
-// 16 bits, forward and backward, 127 us.
+// a warp or, when it is longer than their registers, to a block.  Measured, bf16: 16384 x 4096 with residual forward 82 us (6.5 TB/s),
+// backward 95 us (5.6 TB/s); 8192 x 4096 to 8 bits 52 us (4.5 TB/s: the blocks' barriers); 262144 rows of 128 fp32 values to
+// 16 bits forward 40 us (5.0 TB/s), backward 90 (3.7 TB/s: 368 instructions for a warp's two rows, 58 % of the issue slots at four
+// warps per scheduler; and 888 blocks where 740 fit, so a second wave of a fifth).
+// What is far from its bytes: the backward on an fp32 stream (bf16 x, 16384 x 4096: 270 us where its bytes take 166; held to 64 registers for
+// a second block, for which its ring leaves no room), rows above 8192 (4096 x 16384 bf16: forward 100, backward 131 us, of 83 each; the
+// forms with 32 values a thread spill), and rows that are no multiple of 8 values or not aligned to 16 bytes, which go value by
+// value (16384 x 4095: 208 and 434 us; 262144 rows of 33: 162 and 239).
 #include <cuda_fp8.h>
 
 #include "async_copy.cuh"

@@ -268,7 +268,7 @@ cudaError_t launch_ssm_fwd(const SsmFwdArgs& a, cudaStream_t st) {
     }
     return launch_ssm_fwd_pass<T, K, true>(a, a.nseg, st);
 }
-// States per warp: as few as hold all N.  (Six for 24 states, twelve for 48: 157 and 302 us for 2 x 2048 x 2048 positions and channels, bf16,
+// States per warp: as few as hold all N.  (Six for 24 states, twelve for 48: 157 and 307 us for 2 x 2048 x 2048 positions and channels, bf16,
 // against 210 and 415 with eight and sixteen, which leave the last warp without any.)
 template <typename T>
 cudaError_t launch_ssm_fwd_n(const SsmFwdArgs& a, cudaStream_t st) {

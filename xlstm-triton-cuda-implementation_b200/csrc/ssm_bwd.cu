@@ -15,11 +15,11 @@
 // states run over the warps through shared memory.  No atomics: the same inputs give the same bits.
 //
 // What bounds it: latency.  255 registers allow eight warps per SM, and a warp's two recurrences, exponentials, broadcasts and
-// butterflies are chains: 24 instructions per state and position, issue slots 50 %, shared memory 55 %, exponentials 29 % busy.
-// Measured, bf16, 16 states: 4 x 4096 x 4096 1.79 ms (2.29 with the forward), 2 x 2048 x 4096 0.53 ms.  Tried and slower for the
-// first (forward + backward, ms): four positions at a time (163 registers, more states recomputed) 2.59; four more warps that
-// prepare and finish, as in the forward 2.86; the channel sums through shared memory 2.38; two states per warp and sixteen warps
-// per SM 2.64.
+// butterflies are chains: 24 instructions per state and position; with two blocks on every SM issue slots 47 %, shared memory 56 %,
+// exponentials 30 % busy.  Measured, bf16, 16 states: 4 x 4096 x 4096 1.77 ms (2.27 with the forward), 2 x 2048 x 4096 0.54 ms (0.73).
+// Tried and slower for the first, when it took 2.29 ms with the forward: four positions at a time (163 registers, more states recomputed)
+// 2.59; four more warps that prepare and finish, as in the forward 2.86; the channel sums through shared memory 2.38; two states per
+// warp at 128 registers, sixteen warps per SM 2.64.  More than 32 states, and 17 to 24, spill 36 to 80 bytes a thread.
 #include "async_copy.cuh"
 #include "reduce_rows.cuh"
 #include "ssm_common.cuh"
@@ -454,8 +454,8 @@ struct SsmParamOut {
 
 constexpr size_t SSM_BWD_PART_MAX = 512u << 20;     // bytes of dB, dC partials in scratch at one time (at least one batch entry)
 // Four states per warp and four warps: two CTAs fill an SM's registers.  Where the channels give at most one CTA to an SM, or there are
-// more states, eight warps (with two states each, 4 x 4096 x 4096: 2.69 against 2.33 ms for forward and backward, but
-// 2 x 2048 x 4096: 0.74 against 0.83 ms).
+// more states, eight warps.  (With two states each, so one CTA of eight warps per SM, forward and backward of 4 x 4096 x 4096 take
+// 2.65 against 2.27 ms, but those of 2 x 2048 x 4096 0.73 against 0.81 ms.)
 bool ssm_bwd_wide(const SsmArgs& a) { return a.N > 16 || (a.N > 8 && static_cast<long long>(a.G) * a.tiles_g * a.Bt <= 148); }
 void ssm_bwd_cut(SsmArgs& a) { ssm_cut(a, ssm_bwd_wide(a) ? 1 : 2); }
 

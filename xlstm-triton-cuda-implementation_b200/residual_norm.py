@@ -10,7 +10,7 @@ x: contiguous, float32 / float16 / bfloat16; residual: x's type or float32; weig
 [NH, D] for an x of shape [B, NH, S, D]: a norm of its own for every head of a mixer's result, as ``mlstm_scan`` and
 ``mlstm_matmul`` return it.  What is normalised is the sum as it is returned, rounded to the stream's type, so that the gradients
 are those of the values that the next layer sees.  ``out_dtype``: x's type by default; any type where the stream (x, or
-the residual) is float32.
+the residual) is float32.  Squares are summed in float32, so magnitudes above 1e19 overflow.
 
 Inputs that require gradients get them, through the norm and through the sum.  The quantized form has none: its result feeds an
 8-bit product.  The reference has neither; they stand beside ``output_gate_forward`` in what follows a mixer.
