@@ -121,3 +121,15 @@ def test_convolution_scratch_covers_every_access_width(pkg):
                 need = L.mlstm_conv_bwd_workspace(B, S, C, 4, dt)
                 rc = L.mlstm_conv_bwd(at(base), at(base), at(4096), None, None, at(base), at(4096), None, at(4096), need, B, S, C, 4, dt, dt, 1, None)
                 assert rc not in (0, -5), (dt, B, S, C, base, rc)
+
+
+def test_sizes_that_do_not_fit_are_refused_before_they_become_32_bits(pkg):
+    at = lambda *s: torch.empty(s, device="meta")
+    for shape in ((1, 2 ** 32 + 8, 8), (1, 2 ** 23 + 1, 8), (2 ** 32 + 1, 1, 8), (65536, 1, 8), (1, 1, 2 ** 24 + 1), (1, 1, 2 ** 32 + 8)):
+        with pytest.raises(ValueError, match="at most"):
+            pkg.short_convolution(at(*shape), at(shape[2], 4))
+        if shape[1] != 2 ** 23 + 1:
+            with pytest.raises(ValueError, match="at most"):
+                pkg.state_space_scan(at(*shape), at(*shape), at(shape[2], 16), at(*shape[:2], 16), at(*shape[:2], 16))
+    with pytest.raises(ValueError, match="fewer than"):
+        pkg.state_space_scan(at(1, 2 ** 31 - 32, 8), at(1, 2 ** 31 - 32, 8), at(8, 16), at(1, 2 ** 31 - 32, 16), at(1, 2 ** 31 - 32, 16))

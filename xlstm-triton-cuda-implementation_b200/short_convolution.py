@@ -31,7 +31,9 @@ def _check(x, weight, bias, activation):
     """(device, strides of x or None where it is contiguous)"""
     if x.dim() != 3 or not x.numel():
         raise ValueError("x must have the shape [B, S, C] with at least one of each")
-    C = x.shape[2]
+    B, S, C = x.shape
+    if B > 65535 or S > 1 << 23 or C > 1 << 24:      # (before they become 32 bits)
+        raise ValueError("x must have at most 65535 batch entries, 2^23 positions and 2^24 channels")
     if weight.dim() != 2 or weight.shape[0] != C or not 2 <= weight.shape[1] <= 4:
         raise ValueError("weight must have the shape [C, W] with W = 2, 3 or 4")
     if activation not in _ACTIVATIONS:

@@ -14,8 +14,8 @@ D, dt_bias: [channels], float32; N <= 64.  D, z and dt_bias may be None.  y has 
 ``initial`` ([batch, channels, N] float32) continues an earlier call, ``return_state`` gives the state behind this one, and
 ``state_out`` names the tensor it is written to, which may be ``initial`` itself (a decoding loop in a CUDA graph keeps one
 buffer).  Up to 8 positions take a kernel for decoding, as ``mlstm_chunkwise`` does for its mixer.  A position with delta = 0
-(dt = -inf with ``dt_softplus``) and a finite x leaves the state as it is and gets gradients of 0 for dt and B: so a batch of
-different lengths is padded, on either side.
+(dt = -inf with ``dt_softplus``) and finite values in its other inputs leaves the state as it is and gets gradients of 0 for dt
+and B: so a batch of different lengths is padded, on either side.
 
 Inputs that require gradients get them (no states in that case): the forward then keeps the state in front of every 16
 positions (N / 16 float32 values per element of x) and the backward recomputes what lies between.
@@ -55,6 +55,8 @@ def _check(x, dt, A, B, C, D, z, dt_bias):
     if dt.shape != shape or (z is not None and z.shape != shape):
         raise ValueError("x, dt and z must share the shape [batch, S, channels]")
     b, S, ch = shape
+    if b > 65535 or S >= (1 << 31) - 32 or ch > 1 << 24:      # (before they become 32 bits)
+        raise ValueError("x must have at most 65535 batch entries, 2^24 channels and fewer than 2^31 - 32 positions")
     vectors = B.shape
     if len(vectors) not in (3, 4) or C.shape != vectors or vectors[0] != b or vectors[1] != S:
         raise ValueError("B and C must share the shape [batch, S, N] or [batch, S, G, N]")
