@@ -960,3 +960,47 @@ def test_convolution_of_aligned_channels(pk, dtype, B, S, C, W, bias, silu, init
     """Several channels per thread with every number of taps, with and without silu and bias, in both directions."""
     test_convolution(pk, dtype, B, S, C, W, bias, silu, initial, w32, wide)
     test_convolution_gradients(pk, dtype, B, S, C, W, bias, silu, initial, w32, wide)
+
+
+# ---------------------------------------------------------------------------------------------- combinations of the norm's options
+@pytest.mark.parametrize("D,block", [(64, 32), (96, None), (128, 64), (33, None)])
+def test_quantized_norm_of_every_head(pk, D, block):
+    g = gen(D)
+    h, w, res = torch.randn(2, 3, 41, D, generator=g) * 4, 1 + 0.3 * torch.randn(3, D, generator=g), torch.randn(2, 3, 41, D, generator=g)
+    y = pk.residual_rms_norm(h.cuda(), w.cuda())
+    q, scale = pk.residual_rms_norm_quantized(h.cuda(), w.cuda(), block=block)
+    assert q.shape == h.shape and scale.shape == (2, 3, 41, D // (block or D))
+    assert_eight_bits(q, scale, y, block or D)
+    y, s = pk.residual_rms_norm(h.cuda(), w.cuda(), residual=res.cuda())
+    q, scale, total = pk.residual_rms_norm_quantized(h.cuda(), w.cuda(), residual=res.cuda(), block=block)
+    assert torch.equal(total, s)
+    assert_eight_bits(q, scale, y, block or D)
+
+
+@pytest.mark.parametrize("dtype,wdt,out", [(F16, F16, BF16), (BF16, F32, F16), (BF16, BF16, F32), (F32, F32, F16), (F16, F32, F16)])
+@pytest.mark.parametrize("shape,heads", [((37, 520), 0), ((2, 3, 50, 64), 3), ((5, 1001), 0)])
+def test_norm_of_a_float32_stream_in_every_type(pk, dtype, wdt, out, shape, heads):
+    """A float32 residual stream takes x of any type and gives its norm in any other; gradients of both, through both results."""
+    g = gen(sum(shape))
+    D = shape[-1]
+    x, res = (2 * torch.randn(*shape, generator=g)).to(dtype), 3 * torch.randn(*shape, generator=g)
+    weight = (1 + 0.3 * torch.randn(*((heads, D) if heads else (D,)), generator=g)).to(wdt)
+    dy, ds = torch.randn(*shape, generator=g).to(out), torch.randn(*shape, generator=g)
+    leaves = [cu(t).requires_grad_(True) for t in (x, weight, res)]
+    y, s = pk.residual_rms_norm(leaves[0], leaves[1], residual=leaves[2], out_dtype=out)
+    assert y.dtype == out and s.dtype == F32
+    got = torch.autograd.grad((y, s), leaves, (cu(dy), cu(ds)))
+    v, wl = oo.leaf(s.detach().cpu()), oo.leaf(weight)
+    want = oo.norm(v, wl)[0]
+    off(y, want, oo.HALF_STEP[out], 32 * U * want.abs(), "y")
+    ref = torch.autograd.grad(want, (v, wl), dy.double())
+    # as in test_norm_gradients
+    r = 1 / torch.sqrt(v.detach().square().mean(-1, keepdim=True) + 1e-6)
+    u = dy.double().abs() * (weight.double().abs()[:, None] if heads else weight.double().abs())
+    mag = r * (u + v.detach().abs() * r * r * (u * v.detach().abs()).mean(-1, keepdim=True)) + ds.double().abs()
+    dv = ref[0] + ds.double()
+    off(got[0], dv, oo.HALF_STEP[dtype], 64 * U * mag, "dx")
+    off(got[2], dv, U, 64 * U * mag, "dresidual")
+    lost = (dy.double() * v.detach() * r).abs()
+    lost = lost.sum((0, 2)) if heads else lost.reshape(-1, D).sum(0)
+    off(got[1], ref[1], oo.HALF_STEP[wdt], (s.numel() / D / 100 + 300) * U * lost, "dweight")
